@@ -193,6 +193,50 @@ TK_API int tk_kv_append(const void* k, int64_t k_tok_stride, const void* v, int6
                         int start_pos, int dtype, void* stream);
 
 /*
+ * The 8-bit KV cache. Per sequence and kv head, blocks of 32 tokens: codes (TK_KV8_E4M3 or
+ * TK_KV8_INT8), one fp32 scale for the block's keys and one for its values (a / M with a the
+ * largest magnitude, at least 2^-60, M = 448 or 127; code = rn(x * (M * (1 / a))); NaN with codes
+ * 0 if the block holds a value that is not finite), and the rows of the block that is not yet
+ * complete in 16 bits:
+ *   k_cache, v_cache [batch, num_kv_heads, num_blocks, 32 * head_dim] bytes
+ *   scales           [batch, num_kv_heads, num_blocks, 2] fp32 (keys, values), 8-byte aligned
+ *   tail             [batch, num_kv_heads, 2 (keys, values), 32, head_dim] of dtype
+ * Order of a block's codes: keys [j=4][h=head_dim/64][n=8][q=4][i=16] are token 8(n/2)+2j+n%2,
+ * column 64h+16q+i; values [m=head_dim/16][r=8][q=4][e=2][t=8] are token 8q+t, column 16m+8e+r.
+ * No reference counterpart (the reference has no KV cache, README.md:102).
+ */
+enum { TK_KV8_E4M3 = 0, TK_KV8_INT8 = 1 };
+
+/*
+ * Append S rows of k (already rotated) and v per sequence at start_pos: blocks that they complete
+ * are quantised, the rows of the block that stays open go to the tail. The rows of the open block
+ * below start_pos must be in the tail, as earlier calls left them.
+ */
+TK_API int tk_kv8_append(const void* k, int64_t k_tok_stride, const void* v, int64_t v_tok_stride, void* k_cache,
+                         void* v_cache, float* scales, void* tail, int num_blocks, int format, int batch, int seq,
+                         int num_kv_heads, int head_dim, int start_pos, int dtype, void* stream);
+
+/*
+ * tk_kv_attention over an 8-bit cache: attention of S new tokens per sequence at start_pos ..
+ * start_pos+S-1 against complete blocks (codes), the open block and their own rows (16 bits), then
+ * their append. cos_table / sin_table NULL: q and k are rotated already. start_pos_device: the
+ * position of sequence b is start_pos_device[b * start_pos_step] (step 0 or 1), read at run time; a
+ * position outside the cache or the table records device error 2 and leaves that sequence's out
+ * and cache as they are. workspace: as for tk_kv_attention. One launch for S = 1, two otherwise.
+ */
+TK_API int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride, const void* v,
+                            int64_t v_tok_stride, void* k_cache, void* v_cache, float* scales, void* tail,
+                            int num_blocks, int format, const float* cos_table, const float* sin_table,
+                            int64_t table_rows, void* out, int64_t out_tok_stride, int batch, int seq, int num_heads,
+                            int num_kv_heads, int head_dim, int start_pos, const int* start_pos_device,
+                            int start_pos_step, void* workspace, int64_t workspace_bytes, int dtype, void* stream);
+
+/* Workspace bytes of tk_kv8_attention when start+S <= max_kv (the cache's capacity when the position
+ * comes from device memory). 0: none needed or invalid sizes, -1: no device. */
+TK_API int64_t tk_kv8_attention_workspace(int batch, int num_heads, int num_kv_heads, int head_dim, int seq,
+                                          int max_kv);
+
+/*
  * One decode step of a whole decoder stack in ONE persistent cooperative kernel (batch <= 8
  * sequences, one new token each): for every layer the q|k|v product (attention RMSNorm folded
  * into wq/wk/wv), tk_kv_attention's work, o_proj + residual, gate|up + SwiGLU (FFN RMSNorm folded

@@ -73,6 +73,10 @@ SIGNATURES = {
                         _P, _P, _I64, _I, _P],
     "tk_kv_attention_workspace": [_I, _I, _I, _I, _I, _I],
     "tk_kv_append": [_P, _I64, _P, _I64, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P],
+    "tk_kv8_append": [_P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _I, _P],
+    "tk_kv8_attention": [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _P, _P, _I64, _P, _I64, _I, _I, _I, _I,
+                         _I, _I, _P, _I, _P, _I64, _I, _P],
+    "tk_kv8_attention_workspace": [_I, _I, _I, _I, _I, _I],
     "tk_decode_step_scratch_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
     "tk_decode_step_setup": [ctypes.POINTER(StepLayer), _I, _I, _I, _I, _I, _I, _I, _P, _P, _I64, _I, _P, _P, _F, _I,
                              _P, _I64],
@@ -89,7 +93,8 @@ SIGNATURES = {
 }
 
 # entry points whose return value is not a status
-RESTYPES = {"tk_kv_attention_workspace": _I64, "tk_decode_step_scratch_bytes": _I64, "tk_stack_scratch_bytes": _I64}
+RESTYPES = {"tk_kv_attention_workspace": _I64, "tk_kv8_attention_workspace": _I64,
+            "tk_decode_step_scratch_bytes": _I64, "tk_stack_scratch_bytes": _I64}
 
 _lock = threading.Lock()
 _lib = None

@@ -1,0 +1,30 @@
+// Host-side pieces that the 8-bit KV cache entry points share.
+#pragma once
+
+#include <cuda_runtime.h>
+#include <stdint.h>
+
+namespace tk {
+namespace kv8 {
+
+// The tensors of one layer's 8-bit cache (kv8.cuh).
+struct Cache {
+  void* k;
+  void* v;
+  float* scales;
+  void* tail;
+  int num_blocks;
+  int format;
+};
+
+int check_cache(const char* what, const Cache& c, int batch, int seq, int num_heads, int num_kv_heads, int head_dim,
+                int dtype);
+
+// Append launch; with cos_t the keys are rotated at their positions. The position is start_pos, or
+// start_dev[b * start_step] of sequence b.
+int append(const Cache& c, const void* k, int64_t ks, const void* v, int64_t vs, const float* cos_t,
+           const float* sin_t, int64_t table_rows, int batch, int seq, int num_kv_heads, int head_dim, int start_pos,
+           const int* start_dev, int start_step, int dtype, cudaStream_t st);
+
+}  // namespace kv8
+}  // namespace tk
