@@ -237,6 +237,41 @@ TK_API int64_t tk_kv8_attention_workspace(int batch, int num_heads, int num_kv_h
                                           int max_kv);
 
 /*
+ * One step of beam search. For every sequence b the best num_select of
+ *   c[b, k, v] = scores[b, k] + logits[b, k, v] - logsumexp_v(logits[b, k, :])
+ * over beams k and tokens v, best first, ties by the lower k * vocab + v (within a beam the order is that of
+ * the logits, across beams that of c in fp64). logits: row b * beams + k at row_stride elements, any
+ * alignment; scores [batch, beams] fp32; finished NULL or [batch, beams] bytes: a finished beam's
+ * only candidate is eos_token at its score, its other tokens are -inf. A beam whose score is -inf
+ * or NaN is -inf throughout. NaN logits count as -inf, +inf as the largest finite value. Outputs [batch,
+ * num_select]: scores fp32, beam and token int64. num_select 1..64, at most beams * vocab; beams up
+ * to 1024. workspace: tk_beam_select_workspace() bytes, any contents. No reference counterpart.
+ */
+TK_API int tk_beam_select(const void* logits, int64_t row_stride, const float* scores, const uint8_t* finished,
+                          int64_t eos_token, float* out_scores, int64_t* out_beams, int64_t* out_tokens, int batch,
+                          int beams, int vocab, int num_select, void* workspace, int64_t workspace_bytes, int dtype,
+                          void* stream);
+TK_API int64_t tk_beam_select_workspace(int batch, int beams, int vocab, int num_select);
+
+/*
+ * Reorder a KV cache's rows in place after a beam search step: of each group of `beams` consecutive rows, row i
+ * becomes what row parents[g * beams + i] was, positions 0 .. length-1 of all layers. k_cache, v_cache
+ * [layers, groups * beams, num_kv_heads, capacity, head_dim] of dtype. length_device: if not NULL the
+ * length is read from this device int at run time; one outside the cache records device error 2 and
+ * moves nothing. A group with a parent outside 0 .. beams-1 records device error 4 and stays as it
+ * is. beams up to 32.
+ */
+TK_API int tk_kv_reorder(void* k_cache, void* v_cache, const int64_t* parents, int layers, int groups, int beams,
+                         int num_kv_heads, int capacity, int head_dim, int length, const int* length_device,
+                         int dtype, void* stream);
+
+/* The same for an 8-bit cache (each of its tensors with a leading [layers] dimension): whole blocks, their scales
+ * and the length % 32 rows of the tail. */
+TK_API int tk_kv8_reorder(void* k_cache, void* v_cache, float* scales, void* tail, const int64_t* parents, int layers,
+                          int groups, int beams, int num_kv_heads, int num_blocks, int head_dim, int length,
+                          const int* length_device, void* stream);
+
+/*
  * One decode step of a whole decoder stack in ONE persistent cooperative kernel (batch <= 8
  * sequences, one new token each): for every layer the q|k|v product (attention RMSNorm folded
  * into wq/wk/wv), tk_kv_attention's work, o_proj + residual, gate|up + SwiGLU (FFN RMSNorm folded

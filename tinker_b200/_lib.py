@@ -77,6 +77,10 @@ SIGNATURES = {
     "tk_kv8_attention": [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _P, _P, _I64, _P, _I64, _I, _I, _I, _I,
                          _I, _I, _P, _I, _P, _I64, _I, _P],
     "tk_kv8_attention_workspace": [_I, _I, _I, _I, _I, _I],
+    "tk_beam_select": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _P, _I64, _I, _P],
+    "tk_beam_select_workspace": [_I, _I, _I, _I],
+    "tk_kv_reorder": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P],
+    "tk_kv8_reorder": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "tk_decode_step_scratch_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],
     "tk_decode_step_setup": [ctypes.POINTER(StepLayer), _I, _I, _I, _I, _I, _I, _I, _P, _P, _I64, _I, _P, _P, _F, _I,
                              _P, _I64],
@@ -94,7 +98,7 @@ SIGNATURES = {
 
 # entry points whose return value is not a status
 RESTYPES = {"tk_kv_attention_workspace": _I64, "tk_kv8_attention_workspace": _I64,
-            "tk_decode_step_scratch_bytes": _I64, "tk_stack_scratch_bytes": _I64}
+            "tk_beam_select_workspace": _I64, "tk_decode_step_scratch_bytes": _I64, "tk_stack_scratch_bytes": _I64}
 
 _lock = threading.Lock()
 _lib = None
@@ -171,7 +175,8 @@ def stream_ptr(device: torch.device) -> int:
 
 def device_error(clear: bool = True) -> int:
     """Sticky device-side error word (0: none; 1: a bounded wait timed out; 2: a device-side
-    position beyond a KV cache or RoPE table; 3: a token id outside the embedding table)."""
+    position beyond a KV cache or RoPE table; 3: a token id outside the embedding table; 4: a
+    reordered row's parent outside its group of beams)."""
     code = _I(0)
     check(lib().tk_device_error(ctypes.byref(code), 1 if clear else 0), "tk_device_error")
     return code.value

@@ -62,6 +62,14 @@ def kv8_attention_workspace(batch: int, num_heads: int, num_kv_heads: int, head_
     return int(n)
 
 
+def _rows(t: torch.Tensor, B: int, S: int, width: int) -> tuple[torch.Tensor, int]:
+    """``_token_stride`` whose copy is also made where the rows do not start on 16 bytes."""
+    t, stride = _token_stride(t, B, S, width)
+    if t.data_ptr() % 16:
+        t, stride = t.clone(memory_format=torch.contiguous_format), width
+    return t, stride
+
+
 def _check_cache(what: str, k_cache, v_cache, scales, tail, batch: int, heads: int, head_dim: int,
                  dtype: torch.dtype) -> tuple[int, int]:
     """(blocks, format code) of a cache that fits the call; raises otherwise."""
@@ -105,9 +113,9 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
     if k.dtype is not q.dtype or v.dtype is not q.dtype:
         raise TypeError("kv8_attention: q, k, v must all be float16 or all bfloat16")
     nb, code = _check_cache("kv8_attention", k_cache, v_cache, scales, tail, B, num_kv_heads, head_dim, q.dtype)
-    q3, qs = _token_stride(q, B, S, num_heads * head_dim)
-    k3, ks = _token_stride(k, B, S, num_kv_heads * head_dim)
-    v3, vs = _token_stride(v, B, S, num_kv_heads * head_dim)
+    q3, qs = _rows(q, B, S, num_heads * head_dim)
+    k3, ks = _rows(k, B, S, num_kv_heads * head_dim)
+    v3, vs = _rows(v, B, S, num_kv_heads * head_dim)
     cos_ptr = sin_ptr = None
     rows = 0
     if cos_table is not None or sin_table is not None:
@@ -165,8 +173,8 @@ def kv8_append(k, v, k_cache, v_cache, scales, tail, start_pos: int = 0) -> None
     B, S = k.shape[0], k.shape[1]
     hkv, D = k_cache.shape[1], k_cache.shape[3] // KV8_BLOCK
     nb, code = _check_cache("kv8_append", k_cache, v_cache, scales, tail, B, hkv, D, k.dtype)
-    k3, ks = _token_stride(k, B, S, hkv * D)
-    v3, vs = _token_stride(v, B, S, hkv * D)
+    k3, ks = _rows(k, B, S, hkv * D)
+    v3, vs = _rows(v, B, S, hkv * D)
     start_pos = int(start_pos)
     if start_pos < 0 or start_pos + S > nb * KV8_BLOCK:
         raise ValueError(f"kv8_append: positions {start_pos}..{start_pos + S - 1} exceed the cache capacity "
