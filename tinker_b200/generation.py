@@ -17,6 +17,12 @@ RMSNorm runs as ONE persistent cooperative kernel per step instead
 (``tk_decode_step``: grid barriers in place of the 5 launches per block), which
 on B200 measures slower than the chained launches (0.63 vs 0.40 ms per token for
 the 268M model at batch 1) and is kept as the alternative.
+
+``KVCache8`` holds the same in 8-bit codes with a scale for each block of 32 tokens and kv head
+(``kernels/kv_cache8.py``): half the bytes of every step's attention, twice the sequences or positions
+in the same memory (``CachedDecoder(cache_dtype=torch.float8_e4m3fn)``). ``beam_search`` keeps the
+beams of each prompt as neighbouring rows of the batch: every step selects over beams and vocabulary in
+one call and moves the cache's rows to the beams they are continued by, in place.
 """
 
 from __future__ import annotations
@@ -27,7 +33,10 @@ import torch.nn as nn
 from tinker_b200 import _lib
 from tinker_b200.fusion import _folded_forward, _folded_weights
 from tinker_b200.kernels._common import call_ctx, stable_weights
-from tinker_b200.kernels.kv_cache import kv_attention_workspace
+from tinker_b200.kernels.beam import beam_select, kv8_reorder, kv_reorder
+from tinker_b200.kernels.kv_cache import kv_append, kv_attention, kv_attention_workspace
+from tinker_b200.kernels.kv_cache8 import (KV8_BLOCK, KV8_FORMATS, kv8_append, kv8_attention, kv8_attention_workspace,
+                                           kv8_empty)
 from tinker_b200.modules.attention import TinKerAttention
 from tinker_b200.modules.normalization import TinKerRMSNorm
 
@@ -44,6 +53,16 @@ class KVCacheLayer:
 
     def workspace(self, seq: int) -> torch.Tensor | None:
         return self.cache.workspace(seq)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, start_pos: int) -> None:
+        """Append rotated keys and values."""
+        kv_append(k, v, self.k, self.v, start_pos)
+
+    def attend(self, q, k, v, cos_table, sin_table, num_heads: int, num_kv_heads: int, head_dim: int, start_pos: int,
+               position: torch.Tensor | None) -> torch.Tensor:
+        """Attention of new tokens (not rotated yet) against this layer, and their append."""
+        return kv_attention(q, k, v, cos_table, sin_table, self.k, self.v, num_heads, num_kv_heads, head_dim,
+                            start_pos, position, self.workspace(q.shape[1]))
 
 
 class KVCache:
@@ -93,6 +112,80 @@ class KVCache:
     def reset(self) -> None:
         self.length = 0
 
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Rows follow their beams: ``kernels.kv_reorder`` over all layers' filled positions."""
+        kv_reorder(self.k, self.v, parents, self.length)
+
+
+class KVCache8Layer:
+    """One layer's view of a ``KVCache8``."""
+
+    def __init__(self, cache: "KVCache8", index: int):
+        self.cache = cache
+        self.index = index
+        self.k, self.v, self.scales, self.tail = (t[index] for t in (cache.k, cache.v, cache.scales, cache.tail))
+
+    def workspace(self, seq: int) -> torch.Tensor | None:
+        return self.cache.workspace(seq)
+
+    def append(self, k: torch.Tensor, v: torch.Tensor, start_pos: int) -> None:
+        """Append rotated keys and values."""
+        kv8_append(k, v, self.k, self.v, self.scales, self.tail, start_pos)
+
+    def attend(self, q, k, v, cos_table, sin_table, num_heads: int, num_kv_heads: int, head_dim: int, start_pos: int,
+               position: torch.Tensor | None) -> torch.Tensor:
+        """Attention of new tokens (not rotated yet) against this layer, and their append."""
+        return kv8_attention(q, k, v, cos_table, sin_table, self.k, self.v, self.scales, self.tail, num_heads,
+                             num_kv_heads, head_dim, start_pos, position, self.workspace(q.shape[1]))
+
+
+class KVCache8:
+    """Keys and values of every layer in 8-bit codes (``kernels/kv_cache8.py``), the tensors of
+    ``kv8_empty`` with a leading layer dimension; the interface of ``KVCache``. ``capacity`` is rounded
+    up to whole blocks of 32 positions. ``length`` may go back to 0, not to any other position inside a
+    complete block (whose 16-bit rows are gone)."""
+
+    def __init__(self, num_layers: int, batch_size: int, num_heads: int, num_kv_heads: int, head_dim: int,
+                 capacity: int, dtype: torch.dtype = torch.float16, device="cuda",
+                 code: torch.dtype = torch.float8_e4m3fn):
+        self.k, self.v, self.scales, self.tail = kv8_empty(batch_size, num_kv_heads, head_dim, capacity, dtype, code,
+                                                           device, layers=num_layers)
+        self.num_heads = num_heads
+        self.num_kv_heads = num_kv_heads
+        self.head_dim = head_dim
+        self.batch_size = batch_size
+        self.capacity = self.k.shape[3] * KV8_BLOCK
+        self.length = 0
+        self.position = torch.zeros(1, dtype=torch.int32, device=device)
+        self._layers = [KVCache8Layer(self, i) for i in range(num_layers)]
+        self._ws: dict = {}
+
+    @property
+    def num_layers(self) -> int:
+        return len(self._layers)
+
+    def layer(self, i: int) -> KVCache8Layer:
+        return self._layers[i]
+
+    def workspace(self, seq: int) -> torch.Tensor | None:
+        """Scratch for ``kv8_attention`` with ``seq`` new tokens at any position (shared by the layers, whose
+        kernels run one after another). One for each ``seq``: a captured step keeps the address of its own."""
+        need = kv8_attention_workspace(self.batch_size, self.num_heads, self.num_kv_heads, self.head_dim, seq,
+                                       self.capacity)
+        if need == 0:
+            return None
+        ws = self._ws.get(seq)
+        if ws is None:
+            ws = self._ws[seq] = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
+        return ws
+
+    def reset(self) -> None:
+        self.length = 0
+
+    def reorder(self, parents: torch.Tensor) -> None:
+        """Rows follow their beams: ``kernels.kv8_reorder`` over all layers' filled positions."""
+        kv8_reorder(self.k, self.v, self.scales, self.tail, parents, self.length)
+
 
 def _find(model: nn.Module, names):
     for n in names:
@@ -103,7 +196,7 @@ def _find(model: nn.Module, names):
 
 
 class CachedDecoder:
-    """Prefill + greedy token-by-token decoding of a patched decoder LM with a KV cache.
+    """Prefill + token-by-token decoding (greedy or beam search) of a patched decoder LM with a KV cache.
 
     ``model`` (or the model an ``optimize`` graph wrapper holds) needs a token embedding
     (``embedding`` / ``embed_tokens`` / ``tok_embeddings``), a ``layers`` list of pre-norm blocks
@@ -112,11 +205,13 @@ class CachedDecoder:
     to the attention modules' RoPE table length. ``fused_step=True`` runs each decode step's
     blocks as one persistent kernel (``tk_decode_step``; raises when the model does not allow it);
     the default keeps the per-block kernels, which are faster on B200. The one-kernel step uses
-    the folded weights as they are at its first step (like a captured graph).
+    the folded weights as they are at its first step (like a captured graph). ``cache_dtype``:
+    ``torch.float8_e4m3fn`` or ``torch.int8`` for an 8-bit cache (``KVCache8``); by default the cache has
+    the model's type.
     """
 
     def __init__(self, model: nn.Module, batch_size: int, capacity: int | None = None, cuda_graph: bool = True,
-                 fused_step: bool = False):
+                 fused_step: bool = False, cache_dtype: torch.dtype | None = None):
         inner = getattr(model, "_model", None)
         if inner is not None and getattr(model, "_graph", None) is not None:
             model = inner  # an optimize() CUDA-graph wrapper: decode with its model
@@ -141,8 +236,14 @@ class CachedDecoder:
         w = self.embedding.weight
         self.device = w.device
         self.batch_size = batch_size
-        self.cache = KVCache(len(attns), batch_size, a0.num_heads, a0.num_kv_heads, a0.head_dim, capacity,
-                             dtype=w.dtype, device=w.device)
+        shape = (len(attns), batch_size, a0.num_heads, a0.num_kv_heads, a0.head_dim, capacity)
+        if cache_dtype in KV8_FORMATS:
+            self.cache = KVCache8(*shape, dtype=w.dtype, device=w.device, code=cache_dtype)
+        elif cache_dtype in (None, w.dtype):
+            self.cache = KVCache(*shape, dtype=w.dtype, device=w.device)
+        else:
+            raise TypeError(f"cache_dtype must be the model's type, float8_e4m3fn or int8, got {cache_dtype}")
+        self.capacity = capacity
         self.cuda_graph = cuda_graph
         self._graph = None
         self._tokens = None
@@ -167,6 +268,8 @@ class CachedDecoder:
         """Why the one-kernel decode step cannot run this model (None: it can)."""
         a0 = self._attns[0]
         w = self.embedding.weight
+        if isinstance(self.cache, KVCache8):
+            return "the cache must have the model's type"
         if w.dtype not in (torch.float16, torch.bfloat16):
             return "the model dtype must be float16 or bfloat16"
         if self.batch_size > 8:
@@ -257,8 +360,8 @@ class CachedDecoder:
         if tokens.dim() != 2 or tokens.shape[0] != self.batch_size:
             raise ValueError(f"tokens must be [{self.batch_size}, S]")
         S = tokens.shape[1]
-        if self.cache.length + S > self.cache.capacity:
-            raise ValueError(f"{self.cache.length + S} positions exceed the cache capacity {self.cache.capacity}")
+        if self.cache.length + S > self.capacity:
+            raise ValueError(f"{self.cache.length + S} positions exceed the cache capacity {self.capacity}")
         logits = self._forward(tokens, self.cache.length, None)
         self.cache.length += S
         self._position_stale = True
@@ -286,8 +389,8 @@ class CachedDecoder:
         """Append one token per sequence (``tokens`` [batch] or [batch, 1]); returns the logits of
         that position, [batch, vocab] (a buffer the next step overwrites when graphs are used)."""
         tokens = tokens.reshape(self.batch_size, 1)
-        if self.cache.length + 1 > self.cache.capacity:
-            raise ValueError(f"the cache is full ({self.cache.capacity} positions)")
+        if self.cache.length + 1 > self.capacity:
+            raise ValueError(f"the cache is full ({self.capacity} positions)")
         if not self.cuda_graph:
             if self.fused_step:  # the one-kernel step reads the position from device memory
                 self.cache.position.fill_(self.cache.length)
@@ -321,6 +424,49 @@ class CachedDecoder:
                 break
             logits = self.decode(nxt)
         return torch.stack(out, dim=1) if out else torch.empty(self.batch_size, 0, dtype=torch.long)
+
+    @torch.no_grad()
+    def beam_search(self, prompt: torch.Tensor, num_beams: int, max_new_tokens: int, eos_token_id: int | None = None,
+                    length_penalty: float = 0.0) -> tuple[torch.Tensor, torch.Tensor]:
+        """Beam search from ``prompt`` [prompts, S] (``batch_size`` = prompts * num_beams) into an empty cache.
+
+        Each step keeps the ``num_beams`` best continuations of every prompt by the sum of their
+        log-probabilities; a beam that has produced ``eos_token_id`` keeps its score and is continued by
+        that token alone. Returns ``(tokens, scores)``: new token ids [prompts, num_beams, n] (CPU), best
+        beam first, n <= max_new_tokens (fewer once all beams have ended), and float32 scores [prompts,
+        num_beams], the sum of log-probabilities divided by the number of tokens up to and including the end
+        token to the power ``length_penalty``."""
+        if prompt.dim() != 2 or num_beams < 1 or prompt.shape[0] * num_beams != self.batch_size:
+            raise ValueError(f"prompt must be [prompts, S] with prompts * num_beams = {self.batch_size}")
+        if num_beams > 32:
+            raise ValueError("at most 32 beams")
+        P, K = prompt.shape[0], num_beams
+        self.reset()
+        seqs = torch.empty(P, K, 0, dtype=torch.long, device=self.device)
+        # the beams of a prompt start equal, so all but the first are out of the first selection
+        scores = torch.full((P, K), float("-inf"), dtype=torch.float32, device=self.device)
+        scores[:, 0] = 0
+        finished = None if eos_token_id is None else torch.zeros(P, K, dtype=torch.bool, device=self.device)
+        logits = self.prefill(prompt.to(self.device).repeat_interleave(K, 0)) if max_new_tokens > 0 else None
+        for i in range(max_new_tokens):
+            scores, parents, tokens = beam_select(logits.reshape(P, K, -1), scores, K, finished, eos_token_id)
+            seqs = torch.cat([seqs.gather(1, parents[..., None].expand(-1, -1, seqs.shape[2])), tokens[..., None]], 2)
+            if finished is not None:
+                finished = finished.gather(1, parents) | (tokens == eos_token_id)
+                if bool(finished.all()):
+                    break
+            if i + 1 < max_new_tokens:
+                self.cache.reorder(parents)
+                logits = self.decode(tokens.reshape(-1))
+        if length_penalty and seqs.shape[2]:
+            n = torch.full((P, K), seqs.shape[2], device=self.device)
+            if eos_token_id is not None:
+                end = seqs == eos_token_id
+                n = torch.where(end.any(2), end.int().argmax(2) + 1, n)
+            scores = scores / n.float() ** length_penalty
+            scores, order = scores.sort(dim=1, descending=True, stable=True)
+            seqs = seqs.gather(1, order[..., None].expand_as(seqs))
+        return seqs.cpu(), scores
 
     def release(self) -> None:
         """Drop the captured graph (and its memory pool) and the one-kernel step's scratch."""

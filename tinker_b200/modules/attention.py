@@ -16,7 +16,6 @@ import torch.nn as nn
 
 from tinker_b200.kernels.fused_attention import causal_attention, fused_attention, precompute_rope_tables
 from tinker_b200.kernels.gemm import linear, linear_rope
-from tinker_b200.kernels.kv_cache import kv_append, kv_attention
 from tinker_b200 import torch_ops
 from tinker_b200.modules._roles import attention_projections
 
@@ -79,7 +78,7 @@ class TinKerAttention(nn.Module):
                 kv_cache=None, position: torch.Tensor | None = None) -> torch.Tensor:
         """forward pass; with ``residual`` the o_proj epilogue adds it to the output.
 
-        ``kv_cache`` (a ``KVCacheLayer``): x holds the tokens at positions ``start_pos ..`` (or from
+        ``kv_cache`` (a ``KVCacheLayer`` or ``KVCache8Layer``): x holds the tokens at positions ``start_pos ..`` (or from
         the device int32 ``position[0]`` on), which attend to the cached positions before them and
         are appended to the cache."""
         if kv_cache is not None:
@@ -103,7 +102,8 @@ class TinKerAttention(nn.Module):
 
         A prompt at position 0 with more than ``PROMPT_MIN_ROWS`` query rows per kv head takes the
         tensor-core path (RoPE in the projection epilogue, causal attention, cache append);
-        everything else, decode steps included, one ``kv_attention`` kernel."""
+        everything else, decode steps included, the cache's own attention (one ``kv_attention`` launch, or
+        ``kv8_attention`` for an 8-bit cache)."""
         if (x.dim() != 3 or self.cos_table.dtype != torch.float32 or self.sin_table.dtype != torch.float32
                 or self.head_dim not in (64, 128)):
             raise ValueError("KV-cache attention needs x [batch, seq, hidden], float32 RoPE tables and "
@@ -118,12 +118,11 @@ class TinKerAttention(nn.Module):
                               l2_prefetch=l2_prefetch)
             k, v = qkv[..., hq:hq + hkv], qkv[..., hq + hkv:]
             a = causal_attention(qkv[..., :hq], k, v, self.num_heads, self.num_kv_heads, self.head_dim)
-            kv_append(k, v, kv_cache.k, kv_cache.v, 0)
+            kv_cache.append(k, v, 0)
             return a
         qkv = linear(x, wq, wk, wv, **norm, l2_prefetch=l2_prefetch)
-        return kv_attention(qkv[..., :hq], qkv[..., hq:hq + hkv], qkv[..., hq + hkv:], self.cos_table,
-                            self.sin_table, kv_cache.k, kv_cache.v, self.num_heads, self.num_kv_heads,
-                            self.head_dim, start_pos, position, kv_cache.workspace(S))
+        return kv_cache.attend(qkv[..., :hq], qkv[..., hq:hq + hkv], qkv[..., hq + hkv:], self.cos_table,
+                               self.sin_table, self.num_heads, self.num_kv_heads, self.head_dim, start_pos, position)
 
     @classmethod
     def from_module(cls, source: nn.Module, rope_theta: float = 10000.0, max_seq_len: int = 2048) -> "TinKerAttention":
