@@ -5,21 +5,26 @@
 // call's own rows in 16 bits. q is rotated in fp32 and not rounded, k is rotated and rounded to the model type (what
 // the cache keeps), o = softmax(q k^T / sqrt(D)) v, rounded once. Then the new rows are appended.
 //
-// One launch for the attention: a CTA takes a range of 32-key tiles of one (sequence, kv head, 8 query rows). Each of
-// its warps runs the products of its own tiles on m16n8k16 with f16 operands and fp32 sums:
+// Products: m16n8k16 with f16 operands and fp32 sums, a warp for each tile of 32 keys.
 //   * codes are exact in f16, so are 16-bit rows times a power of two that brings the tile's largest magnitude to
 //     [2^14, 2^15) (bf16; its 8 bits stay whole for 28 binades below that);
-//   * the 8 query rows fill rows 0-7 of the A operand with f16(q), rows 8-15 with the remainder q - f16(q), likewise
-//     the probabilities: the products lose nothing to 16-bit operands and the rows that GQA leaves unused are free;
+//   * the 8 query rows of a unit (one sequence, kv head and block of rows) fill rows 0-7 of the A operand with
+//     f16(q), rows 8-15 with the remainder q - f16(q), likewise the probabilities: nothing is lost to 16-bit operands,
+//     and the rows that GQA leaves unused are free;
 //   * the scale of a block's values goes into the exponent: with x = s * scale_k / sqrt(D) * log2 e, a weight is
 //     w = 2^(x + log2 scale_v - m), m the running maximum of that sum, O = sum w * code, and the softmax's
 //     denominator is sum w / scale_v. So O needs no pass per block, w stays in [0, 1], and the rounding of log2
 //     scale_v cancels between numerator and denominator.
-// The warps' (m, l, O) rows are merged in shared memory; with the key axis split over CTAs, each stores its rows
-// and the last to arrive (a counter, which it returns to zero) merges them in the order of the chunks, so results do
-// not depend on the order of arrival. For S = 1 the warp that holds the open block also appends the row, or encodes
-// the block if the row completes it (no CTA of the launch reads that block from the cache); for S > 1 a second launch
-// appends, since other CTAs still read the tail.
+//
+// Division of the work: all units' tiles in one line (a 16-bit tile counts TAIL_WEIGHT), cut into equal pieces, one
+// for each CTA that fits on the GPU at once. So long and short sequences, few units and many, keep every SM busy to
+// the end. A piece covers parts of one or more units; a unit that lies in several pieces is merged by the last of
+// their CTAs to arrive (a counter, which it returns to zero), in the order of the pieces, so results do not depend on
+// the order of arrival. No CTA waits for another. With little work the pieces keep PIECE_MIN tiles and begin at units.
+// Every warp of a CTA copies its tiles ahead into a ring of its own in shared memory (cp.async); the warps' (m, l, O)
+// rows are merged there. For S = 1 the warp that holds the open block also appends the row, or encodes the block if
+// the row completes it (nothing in the launch reads that block from the cache); for S > 1 a second launch appends,
+// since other CTAs still read the tail.
 #include <algorithm>
 #include <string>
 
@@ -32,8 +37,9 @@ namespace kv8 {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int ROWS = 8;         // query rows of a CTA
-constexpr int CHUNK_TILES = 8;  // tiles of a CTA at the finest split of the key axis
+constexpr int ROWS = 8;         // query rows of a unit
+constexpr int TAIL_WEIGHT = 3;  // tiles that one 16-bit tile takes as long as
+constexpr int PIECE_MIN = 16;   // weight of a piece when there is little work
 
 struct AttnParams {
   const void* q;
@@ -56,12 +62,21 @@ struct AttnParams {
   int start_pos;
   const int* start_dev;
   int start_step;
-  int n_rb, n_chunks;
+  int n_rb, batch;
   float scale_log2;
-  int* counters;
-  float2* part_ml;
-  float* part_o;
+  int* counters;   // [CTAs], zero between launches
+  float2* part_ml;  // [CTAs][2][ROWS]: the unit that goes on from the piece before, the one that the next goes on with
+  float* part_o;    // [CTAs][2][ROWS][D]
 };
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_async_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
 
 __device__ __forceinline__ void mma16816(float (&c)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3,
                                          uint32_t b0, uint32_t b1) {
@@ -160,357 +175,486 @@ __device__ __forceinline__ void attend_tile(Rows<D>& st, const uint32_t (&qf)[D 
 
 template <int D>
 struct Smem {
-  static constexpr int TILE = BLOCK * D * 2;             // a 16-bit tile of keys or values
-  static constexpr int STAGE = 2 * TILE;                 // per warp
-  static constexpr int ML = WARPS * ROWS * 8;            // merge, over the stages: float2 [WARPS][ROWS]
-  static constexpr int O = ML;                           // float [WARPS][ROWS][D]
-  static constexpr int FLAG = WARPS * STAGE;
+  static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int HALF = BLOCK * D;                       // a block's keys or values
+  static constexpr int RING = STAGES * 2 * HALF;               // of one warp
+  static constexpr int TAIL = WARPS * RING;                    // a 16-bit tile: keys, then values
+  static constexpr int FLAG = TAIL + 2 * BLOCK * D * 2;
   static constexpr int TOTAL = FLAG + 16;
-  static_assert(O + WARPS * ROWS * D * 4 <= FLAG, "the merge must fit in the stages");
+  static constexpr int O = WARPS * ROWS * 8;                   // merge, over the rings: float2 [WARPS][ROWS], then
+  static_assert(O + WARPS * ROWS * D * 4 <= TAIL, "the merge must fit in the rings");  // float [WARPS][ROWS][D]
 };
 
+// The pieces: unit u of sequence b (of `per_b` units) has weight(b); prefix sums place it on the line. Uniform
+// positions need no sums.
+struct Line {
+  int64_t total;  // weight of all units
+  int64_t piece;  // weight of a CTA's piece
+  bool padded;    // units begin at pieces
+};
+
+__device__ __forceinline__ int64_t unit_weight(int start, int seq, int64_t piece_min) {
+  const int n8 = start / BLOCK;
+  const int64_t w = n8 + static_cast<int64_t>(TAIL_WEIGHT) * ((start % BLOCK + seq + BLOCK - 1) / BLOCK);
+  return piece_min > 1 ? (w + piece_min - 1) / piece_min * piece_min : w;
+}
+
+// A position that does not fit has no weight: its sequence is left as it is.
+__device__ __forceinline__ int position_of(const AttnParams& p, int b) {
+  const int start = p.start_dev ? __ldcg(p.start_dev + static_cast<int64_t>(b) * p.start_step) : p.start_pos;
+  const int64_t end = static_cast<int64_t>(start) + p.seq;
+  return start < 0 || end > static_cast<int64_t>(p.num_blocks) * BLOCK || (p.cos_t && end > p.table_rows) ? -1 : start;
+}
+
 template <int DT, int FMT, int D>
-__global__ void __launch_bounds__(THREADS) kv8_attention_kernel(const AttnParams p) {
+__global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ int64_t sum_s[2][WARPS];
   using S = Smem<D>;
   using T = typename Dt<DT>::T;
   constexpr int C16 = D / 8;
   constexpr int H = D / 64;
-  pdl_wait();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int kvh = blockIdx.y / p.n_rb, rb = blockIdx.y % p.n_rb, b = blockIdx.z;
-  const int unit = blockIdx.z * gridDim.y + blockIdx.y;
-  const int start = p.start_dev ? __ldcg(p.start_dev + static_cast<int64_t>(b) * p.start_step) : p.start_pos;
-  const int64_t end = static_cast<int64_t>(start) + p.seq;
-  if (start < 0 || end > static_cast<int64_t>(p.num_blocks) * BLOCK || (p.cos_t && end > p.table_rows)) {
-    if (threadIdx.x == 0 && blockIdx.x == 0 && blockIdx.y == 0) record_device_error(TK_DEVERR_POSITION);
-    return;
-  }
-  const int open = start % BLOCK, n8 = start / BLOCK;
-  const int n_tiles = n8 + (open + p.seq + BLOCK - 1) / BLOCK;
-  const int n_chunks = min(p.n_chunks, (n_tiles + CHUNK_TILES - 1) / CHUNK_TILES);
-  const int chunk = blockIdx.x;
-  if (chunk >= n_chunks) return;
-  const int lo = static_cast<int>(static_cast<int64_t>(n_tiles) * chunk / n_chunks);
-  const int hi = static_cast<int>(static_cast<int64_t>(n_tiles) * (chunk + 1) / n_chunks);
-  const int64_t bh = static_cast<int64_t>(b) * p.num_kv_heads + kvh;
-  const uint8_t* kc = p.kc + bh * p.num_blocks * (BLOCK * D);
-  const uint8_t* vc = p.vc + bh * p.num_blocks * (BLOCK * D);
-  const float2* scales = reinterpret_cast<const float2*>(p.scales) + bh * p.num_blocks;
-
-  // this lane's share of query row r: rotated, brought to the f16 range, split in two
   const int r = lane >> 2, q = lane & 3;
-  const int gr = rb * ROWS + r;
-  int qpos = -1;  // a padding row sees no key of the 16-bit tiles, and its zeros harm nothing in the others
-  uint32_t qf[H * 4][4];
-  float cq;
+  const int per_b = p.num_kv_heads * p.n_rb;
+  const int cta = blockIdx.x, ctas = gridDim.x;
+  pdl_wait();
+
+  // the line: its length exact and padded, then this CTA's piece
+  const bool ragged = p.start_dev && p.start_step;
+  const int common = ragged ? 0 : position_of(p, 0);
+  Line line;
   {
-    float f[H][16];
-    float amax = 0.f;
+    int64_t exact = 0, padded = 0;
+    bool bad = false;
+    if (!ragged) {
+      bad = common < 0;
+      exact = bad ? 0 : unit_weight(common, p.seq, 1) * p.batch;
+      padded = bad ? 0 : unit_weight(common, p.seq, PIECE_MIN) * p.batch;
+    } else {
+      for (int b = threadIdx.x; b < p.batch; b += THREADS) {
+        const int s = position_of(p, b);
+        bad |= s < 0;
+        exact += s < 0 ? 0 : unit_weight(s, p.seq, 1);
+        padded += s < 0 ? 0 : unit_weight(s, p.seq, PIECE_MIN);
+      }
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+      for (int o = 16; o > 0; o >>= 1) {
+        exact += __shfl_xor_sync(0xffffffffu, exact, o);
+        padded += __shfl_xor_sync(0xffffffffu, padded, o);
+      }
+      if (lane == 0) sum_s[0][warp] = exact, sum_s[1][warp] = padded;
+      __syncthreads();
+      exact = padded = 0;
 #pragma unroll
-      for (int i = 0; i < 16; ++i) f[h][i] = 0.f;
-    if (gr < p.rows) {
-      const int s = gr / p.groups, head = kvh * p.groups + gr % p.groups;
-      qpos = start + s;
-      const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.seq + s) * p.qs +
-                     static_cast<int64_t>(head) * D;
+      for (int w = 0; w < WARPS; ++w) exact += sum_s[0][w], padded += sum_s[1][w];
+    }
+    if (bad && cta == 0) record_device_error(TK_DEVERR_POSITION);
+    exact *= per_b;
+    padded *= per_b;
+    line.padded = padded <= static_cast<int64_t>(ctas) * PIECE_MIN;
+    line.total = line.padded ? padded : exact;
+    line.piece = line.padded ? PIECE_MIN : (exact + ctas - 1) / ctas;
+  }
+  const int64_t from = line.piece * cta, to = min(line.total, from + line.piece);
+  if (from >= to) return;
+
+  // the sequence that `from` lies in, and where it begins
+  int b = 0;
+  int64_t at = 0;  // the line position of sequence b's first unit
+  const int64_t pad = line.padded ? PIECE_MIN : 1;
+  if (!ragged) {
+    const int64_t w = unit_weight(common, p.seq, pad) * per_b;
+    b = static_cast<int>(from / w);
+    at = b * w;
+  } else {
+    // a warp at a time over 32 sequences; all warps do the same
+    for (int b0 = 0;; b0 += 32) {
+      const int s = b0 + lane < p.batch ? position_of(p, b0 + lane) : -1;
+      const int64_t mine = s < 0 ? 0 : unit_weight(s, p.seq, pad) * per_b;
+      int64_t upto = mine;
+#pragma unroll
+      for (int o = 1; o < 32; o <<= 1) {
+        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        if (lane >= o) upto += v;
+      }
+      const uint32_t past = __ballot_sync(0xffffffffu, at + upto > from);
+      if (past) {
+        const int i = __ffs(past) - 1;
+        b = b0 + i;
+        at += __shfl_sync(0xffffffffu, upto - mine, i);
+        break;
+      }
+      at += __shfl_sync(0xffffffffu, upto, 31);
+    }
+  }
+
+  const uint32_t ring = smem_u32(smem) + warp * S::RING;
+  const uint8_t* ring_p = smem + warp * S::RING;
+  int64_t here = from;
+  while (here < to) {
+    const int start = ragged ? position_of(p, b) : common;
+    const int64_t w_unit = start < 0 ? 0 : unit_weight(start, p.seq, pad);
+    if (here >= at + w_unit * per_b) {  // on to the next sequence (one without a valid position has no weight)
+      at += w_unit * per_b;
+      ++b;
+      continue;
+    }
+    const int y = static_cast<int>((here - at) / w_unit);
+    const int64_t unit_at = at + y * w_unit;                       // line position of the unit
+    const int kvh = y / p.n_rb, rb = y % p.n_rb;
+    const int open = start % BLOCK, n8 = start / BLOCK, n16 = (open + p.seq + BLOCK - 1) / BLOCK;
+    const int64_t end = static_cast<int64_t>(start) + p.seq;
+    const int64_t lo_w = here - unit_at, hi_w = min(to - unit_at, w_unit);
+    here = unit_at + hi_w;
+    const int64_t tail_w = static_cast<int64_t>(TAIL_WEIGHT) * n16;
+    // 16-bit tiles whose first weight lies in the piece, then blocks
+    const int t16_lo = static_cast<int>(min(static_cast<int64_t>(n16), (lo_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT));
+    const int t16_hi = static_cast<int>(min(static_cast<int64_t>(n16), (hi_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT));
+    const int lo = static_cast<int>(min(static_cast<int64_t>(n8), max(lo_w - tail_w, int64_t(0))));
+    const int hi = static_cast<int>(min(static_cast<int64_t>(n8), max(hi_w - tail_w, int64_t(0))));
+    const int64_t bh = static_cast<int64_t>(b) * p.num_kv_heads + kvh;
+    const uint8_t* kc = p.kc + bh * p.num_blocks * S::HALF;
+    const uint8_t* vc = p.vc + bh * p.num_blocks * S::HALF;
+    const float2* scales = reinterpret_cast<const float2*>(p.scales) + bh * p.num_blocks;
+
+    // this warp's blocks: in rounds of one for each warp, without warp 0 for as long as it has 16-bit tiles
+    const int skip = TAIL_WEIGHT * (t16_hi - t16_lo), n = hi - lo;
+    auto tile_of = [&](int i) {
+      return lo + (i < skip ? i * (WARPS - 1) + warp - 1 : skip * (WARPS - 1) + (i - skip) * WARPS + warp);
+    };
+    const int i0 = warp == 0 ? skip : 0;
+    int n_my = i0;
+    {
+      const int free_first = skip * (WARPS - 1);
+      if (n <= free_first) {
+        if (warp > 0) n_my = (n - (warp - 1) + WARPS - 2) / (WARPS - 1);
+      } else {
+        n_my = skip + max(0, (n - free_first - warp + WARPS - 1) / WARPS);
+      }
+      n_my = max(n_my, i0);
+    }
+    const T* tail = reinterpret_cast<const T*>(p.tail) + bh * 2 * BLOCK * D;
+    uint8_t* ktile = smem + S::TAIL;
+    uint8_t* vtile = ktile + BLOCK * D * 2;
+
+    auto copy_tail = [&](int t) {  // the rows of 16-bit tile t that the tail holds
+      if (t > 0) return;
+#pragma unroll 4
+      for (int idx = lane; idx < open * C16; idx += 32) {
+        const int row = idx / C16, c = idx % C16;
+        cp_async16(smem_u32(ktile) + tile_off<D>(row, c), tail + row * D + c * 8);
+        cp_async16(smem_u32(vtile) + tile_off<D>(row, c), tail + (BLOCK + row) * D + c * 8);
+      }
+    };
+    auto issue = [&](int i) {  // this warp's i-th block into its ring
+      if (i < n_my) {
+        const int64_t t = tile_of(i);
+        const uint32_t dst = ring + ((i - i0) % S::STAGES) * (2 * S::HALF) + lane * 16;
+        const uint8_t* ks = kc + t * S::HALF + lane * 16;
+        const uint8_t* vs = vc + t * S::HALF + lane * 16;
+#pragma unroll
+        for (int j = 0; j < S::HALF / 512; ++j) cp_async16(dst + j * 512, ks + j * 512);
+#pragma unroll
+        for (int j = 0; j < S::HALF / 512; ++j) cp_async16(dst + S::HALF + j * 512, vs + j * 512);
+      }
+      cp_async_commit();
+    };
+    if (warp == 0 && t16_lo < t16_hi) copy_tail(t16_lo);
+    cp_async_commit();
+#pragma unroll
+    for (int i = 0; i < S::STAGES - 1; ++i) issue(i0 + i);
+
+    // this lane's share of query row r: rotated, brought to the f16 range, split in two
+    const int gr = rb * ROWS + r;
+    int qpos = -1;  // a padding row sees no key of the 16-bit tiles, and its zeros harm nothing in the others
+    uint32_t qf[H * 4][4];
+    float cq;
+    {
+      float f[H][16];
+      float amax = 0.f;
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int c = 8 * h + 2 * q + e;
-          const uint4 x = __ldcg(reinterpret_cast<const uint4*>(row) + c);
-          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-          float cc[4] = {1.f, 1.f, 1.f, 1.f}, ss[4] = {0.f, 0.f, 0.f, 0.f};
-          if (p.cos_t) {
-            const int64_t at = static_cast<int64_t>(qpos) * (D / 2) + c * 4;
-            const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos_t + at));
-            const float4 d = __ldg(reinterpret_cast<const float4*>(p.sin_t + at));
-            cc[0] = a.x, cc[1] = a.y, cc[2] = a.z, cc[3] = a.w;
-            ss[0] = d.x, ss[1] = d.y, ss[2] = d.z, ss[3] = d.w;
-          }
+        for (int i = 0; i < 16; ++i) f[h][i] = 0.f;
+      if (gr < p.rows) {
+        const int s = gr / p.groups, head = kvh * p.groups + gr % p.groups;
+        qpos = start + s;
+        const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.seq + s) * p.qs +
+                       static_cast<int64_t>(head) * D;
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const float2 v = unpack2<DT>(w[i]);
-            f[h][8 * e + 2 * i] = v.x * cc[i] - v.y * ss[i];
-            f[h][8 * e + 2 * i + 1] = v.x * ss[i] + v.y * cc[i];
+        for (int h = 0; h < H; ++h)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            const int c = 8 * h + 2 * q + e;
+            const uint4 x = __ldcg(reinterpret_cast<const uint4*>(row) + c);
+            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
+            float cc[4] = {1.f, 1.f, 1.f, 1.f}, ss[4] = {0.f, 0.f, 0.f, 0.f};
+            if (p.cos_t) {
+              const int64_t ang = static_cast<int64_t>(qpos) * (D / 2) + c * 4;
+              const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos_t + ang));
+              const float4 d = __ldg(reinterpret_cast<const float4*>(p.sin_t + ang));
+              cc[0] = a.x, cc[1] = a.y, cc[2] = a.z, cc[3] = a.w;
+              ss[0] = d.x, ss[1] = d.y, ss[2] = d.z, ss[3] = d.w;
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float2 v = unpack2<DT>(w[i]);
+              f[h][8 * e + 2 * i] = v.x * cc[i] - v.y * ss[i];
+              f[h][8 * e + 2 * i + 1] = v.x * ss[i] + v.y * cc[i];
+            }
           }
+      }
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(f[h][i]));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
+      amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
+      const float up = to_f16_range(__float_as_uint(amax));
+      cq = p.scale_log2 / up;
+#pragma unroll
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int t = 0; t < 4; ++t) {
+          split2(f[h][4 * t] * up, f[h][4 * t + 1] * up, qf[h * 4 + t][0], qf[h * 4 + t][1]);
+          split2(f[h][4 * t + 2] * up, f[h][4 * t + 3] * up, qf[h * 4 + t][2], qf[h * 4 + t][3]);
         }
     }
+
+    Rows<D> st;
+    st.m = -INFINITY;
+    st.l = 0.f;
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+    for (int n2 = 0; n2 < D / 8; ++n2)
 #pragma unroll
-      for (int i = 0; i < 16; ++i) amax = fmaxf(amax, fabsf(f[h][i]));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
-    amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
-    const float up = to_f16_range(__float_as_uint(amax));
-    cq = p.scale_log2 / up;
-#pragma unroll
-    for (int h = 0; h < H; ++h)
-#pragma unroll
-      for (int t = 0; t < 4; ++t) {
-        split2(f[h][4 * t] * up, f[h][4 * t + 1] * up, qf[h * 4 + t][0], qf[h * 4 + t][1]);
-        split2(f[h][4 * t + 2] * up, f[h][4 * t + 3] * up, qf[h * 4 + t][2], qf[h * 4 + t][3]);
+      for (int i = 0; i < 4; ++i) st.o[n2][i] = 0.f;
+
+    // the open block and the new rows: warp 0
+    for (int t = t16_lo; warp == 0 && t < t16_hi; ++t) {
+      if (t > t16_lo) {
+        __syncwarp();
+        copy_tail(t);
       }
-  }
-
-  Rows<D> st;
-  st.m = -INFINITY;
-  st.l = 0.f;
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-    for (int i = 0; i < 4; ++i) st.o[n][i] = 0.f;
-
-  // complete blocks: the next block's keys are loaded once this one's are used, likewise its values
-  const int hi8 = min(hi, n8);
-  const int first = lo + warp;
-  uint4 kr[4][H], vr[D / 16];
-  float2 sc = make_float2(1.f, 1.f);
-  auto load_keys = [&](int t) {
-    const uint4* src = reinterpret_cast<const uint4*>(kc + static_cast<int64_t>(t) * (BLOCK * D)) + lane;
-#pragma unroll
-    for (int j = 0; j < 4; ++j)
-#pragma unroll
-      for (int h = 0; h < H; ++h) kr[j][h] = __ldcg(src + (j * H + h) * 32);
-  };
-  auto load_values = [&](int t) {
-    const uint4* src = reinterpret_cast<const uint4*>(vc + static_cast<int64_t>(t) * (BLOCK * D)) + lane;
-#pragma unroll
-    for (int m = 0; m < D / 16; ++m) vr[m] = __ldcg(src + m * 32);
-  };
-  if (first < hi8) {
-    sc = __ldcg(scales + first);
-    load_keys(first);
-    load_values(first);
-  }
-  for (int t = first; t < hi8; t += WARPS) {
-    const float2 now = sc;
-    const int next = t + WARPS;
-    const bool more = next < hi8;
-    if (more) sc = __ldcg(scales + next);
-    attend_tile<D, false>(
-        st, qf, cq * now.x, __log2f(now.y), 1.f / now.y, lane,
-        [&](int j, int h, uint32_t (&w)[8]) {
-          decode4<FMT>(kr[j][h].x, w[0], w[1]);
-          decode4<FMT>(kr[j][h].y, w[2], w[3]);
-          decode4<FMT>(kr[j][h].z, w[4], w[5]);
-          decode4<FMT>(kr[j][h].w, w[6], w[7]);
-          if (j == 3 && h == H - 1 && more) load_keys(next);
-        },
-        [&](int m, uint32_t (&w)[8]) {
-          decode4<FMT>(vr[m].x, w[0], w[1]);
-          decode4<FMT>(vr[m].y, w[2], w[3]);
-          decode4<FMT>(vr[m].z, w[4], w[5]);
-          decode4<FMT>(vr[m].w, w[6], w[7]);
-          if (m == D / 16 - 1 && more) load_values(next);
-        },
-        [](int) { return true; });
-  }
-
-  // the open block and the new rows
-  for (int t = first; t < hi; t += WARPS) {
-    if (t < n8) continue;
-    const uint32_t ktile = smem_u32(smem) + warp * S::STAGE, vtile = ktile + S::TILE;
-    uint8_t* kp = smem + warp * S::STAGE;
-    uint8_t* vp = kp + S::TILE;
-    const T* tail = reinterpret_cast<const T*>(p.tail) + bh * 2 * BLOCK * D;
-    const int n_rows = min(BLOCK, static_cast<int>(end - static_cast<int64_t>(t) * BLOCK));
-    uint32_t km = 0, vm = 0;
-    __syncwarp();
-#pragma unroll 4
-    for (int i = 0; i < C16; ++i) {
-      const int idx = lane + 32 * i, row = idx / C16, c = idx % C16;
-      const int s = (t - n8) * BLOCK + row - open;  // the call's row, or one of the tail
-      uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-      if (row < n_rows) {
-        if (s < 0) {
-          kx = __ldcg(reinterpret_cast<const uint4*>(tail + row * D) + c);
-          vx = __ldcg(reinterpret_cast<const uint4*>(tail + (BLOCK + row) * D) + c);
-        } else {
-          const int64_t tok = static_cast<int64_t>(b) * p.seq + s;
+      const int n_rows = min(BLOCK, static_cast<int>(end - static_cast<int64_t>(n8 + t) * BLOCK));
+      const int row0 = t == 0 ? open : 0;  // the first row that the call brings
+      for (int idx = lane; idx < (BLOCK - row0) * C16; idx += 32) {
+        const int row = row0 + idx / C16, c = idx % C16;
+        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
+        if (row < n_rows) {
+          const int64_t s = t * BLOCK + row - open, tok = static_cast<int64_t>(b) * p.seq + s;
           kx = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + tok * p.ks +
                                                      static_cast<int64_t>(kvh) * D) + c);
           vx = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + tok * p.vs +
                                                      static_cast<int64_t>(kvh) * D) + c);
           if (p.cos_t) {
-            const int64_t at = (static_cast<int64_t>(start) + s) * (D / 2) + c * 4;
-            rope_chunk<DT>(kx, p.cos_t + at, p.sin_t + at);
+            const int64_t ang = (static_cast<int64_t>(start) + s) * (D / 2) + c * 4;
+            rope_chunk<DT>(kx, p.cos_t + ang, p.sin_t + ang);
           }
         }
+        *reinterpret_cast<uint4*>(ktile + tile_off<D>(row, c)) = kx;
+        *reinterpret_cast<uint4*>(vtile + tile_off<D>(row, c)) = vx;
       }
-      km = amax2(amax2(amax2(amax2(km, kx.x), kx.y), kx.z), kx.w);
-      vm = amax2(amax2(amax2(amax2(vm, vx.x), vx.y), vx.z), vx.w);
-      *reinterpret_cast<uint4*>(kp + tile_off<D>(row, c)) = kx;
-      *reinterpret_cast<uint4*>(vp + tile_off<D>(row, c)) = vx;
-    }
-    km = amax2_warp(km);
-    vm = amax2_warp(vm);
-    __syncwarp();
+      if (t == 0) cp_async_wait<S::STAGES - 1>();  // the tail's rows; the blocks behind them may still be on the way
+      __syncwarp();
+      uint32_t km = 0, vm = 0;
+      if (DT == TK_BF16 || open + p.seq == BLOCK) {
+#pragma unroll 4
+        for (int i = 0; i < C16; ++i) {  // any order of the tile's chunks
+          const uint4 kx = *reinterpret_cast<const uint4*>(ktile + (lane + 32 * i) * 16);
+          const uint4 vx = *reinterpret_cast<const uint4*>(vtile + (lane + 32 * i) * 16);
+          km = amax2(amax2(amax2(amax2(km, kx.x), kx.y), kx.z), kx.w);
+          vm = amax2(amax2(amax2(amax2(vm, vx.x), vx.y), vx.z), vx.w);
+        }
+        km = amax2_warp(km);
+        vm = amax2_warp(vm);
+      }
 
-    // f16 takes its own rows as they are; bf16 rows are brought to its range
-    const float fk = DT == TK_F16 ? 1.f : to_f16_range(km << 16), fv = DT == TK_F16 ? 1.f : to_f16_range(vm << 16);
-    auto to_half = [](uint32_t w, float f) -> uint32_t {
-      if constexpr (DT == TK_F16) {
-        return w;
-      } else {
-        const float2 v = unpack2<DT>(w);
-        return h2_u32(__floats2half2_rn(v.x * f, v.y * f));
+      // f16 takes its own rows as they are; bf16 rows are brought to its range
+      const float fk = DT == TK_F16 ? 1.f : to_f16_range(km << 16), fv = DT == TK_F16 ? 1.f : to_f16_range(vm << 16);
+      auto to_half = [](uint32_t w, float f) -> uint32_t {
+        if constexpr (DT == TK_F16) {
+          return w;
+        } else {
+          const float2 v = unpack2<DT>(w);
+          return h2_u32(__floats2half2_rn(v.x * f, v.y * f));
+        }
+      };
+      attend_tile<D, true>(
+          st, qf, cq / fk, -__log2f(fv), fv, lane,
+          [&](int j, int h, uint32_t (&w)[8]) {
+            const int row = 8 * (r >> 1) + 2 * j + (r & 1);
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              const uint4 x = *reinterpret_cast<const uint4*>(ktile + tile_off<D>(row, 8 * h + 2 * q + e));
+              w[4 * e] = to_half(x.x, fk);
+              w[4 * e + 1] = to_half(x.y, fk);
+              w[4 * e + 2] = to_half(x.z, fk);
+              w[4 * e + 3] = to_half(x.w, fk);
+            }
+          },
+          [&](int m, uint32_t (&w)[8]) {
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              uint32_t x[4];
+              load_column_tokens<D>(smem_u32(vtile), 2 * m + e, lane, x);
+#pragma unroll
+              for (int i = 0; i < 4; ++i) w[4 * e + i] = to_half(x[i], fv);
+            }
+          },
+          [&](int token) { return (n8 + t) * BLOCK + token <= qpos; });
+
+      if (p.seq == 1 && rb == 0) {  // the append of a decode step
+        T* to_row = reinterpret_cast<T*>(p.tail) + bh * 2 * BLOCK * D;
+        if (open < BLOCK - 1) {
+          for (int c = lane; c < 2 * C16; c += 32) {
+            const bool val = c >= C16;
+            const int cc = val ? c - C16 : c;
+            *(reinterpret_cast<uint4*>(to_row + ((val ? BLOCK : 0) + open) * D) + cc) =
+                *reinterpret_cast<const uint4*>((val ? vtile : ktile) + tile_off<D>(open, cc));
+          }
+        } else {
+          const int64_t block = bh * p.num_blocks + n8;
+          const float sk = encode_keys<DT, FMT, D>(p.kc + block * S::HALF, lane, [&](int tok, int c) {
+            return *reinterpret_cast<const uint4*>(ktile + tile_off<D>(tok, c));
+          });
+          const float sv = encode_values<DT, FMT, D>(p.vc + block * S::HALF, lane, smem_u32(vtile), vm);
+          if (lane == 0) reinterpret_cast<float2*>(p.scales)[block] = make_float2(sk, sv);
+        }
       }
+    }
+
+    // complete blocks; lane i keeps the scales of the warp's i-th block of each 32
+    float ks_l = 0.f, lv_l = 0.f, iv_l = 0.f;
+    for (int i = i0; i < n_my; ++i) {
+      if (((i - i0) & 31) == 0 && i + lane < n_my) {
+        const float2 sc = __ldcg(scales + tile_of(i + lane));
+        ks_l = sc.x;
+        lv_l = __log2f(sc.y);
+        iv_l = 1.f / sc.y;
+      }
+      issue(i + S::STAGES - 1);
+      cp_async_wait<S::STAGES - 1>();
+      __syncwarp();  // every lane's copies of block i have landed
+      const uint8_t* kb = ring_p + ((i - i0) % S::STAGES) * (2 * S::HALF) + lane * 16;
+      const uint8_t* vb = kb + S::HALF;
+      const int src = (i - i0) & 31;
+      attend_tile<D, false>(
+          st, qf, cq * __shfl_sync(0xffffffffu, ks_l, src), __shfl_sync(0xffffffffu, lv_l, src),
+          __shfl_sync(0xffffffffu, iv_l, src), lane,
+          [&](int j, int h, uint32_t (&w)[8]) {
+            const uint4 x = *reinterpret_cast<const uint4*>(kb + (j * H + h) * 512);
+            decode4<FMT>(x.x, w[0], w[1]);
+            decode4<FMT>(x.y, w[2], w[3]);
+            decode4<FMT>(x.z, w[4], w[5]);
+            decode4<FMT>(x.w, w[6], w[7]);
+          },
+          [&](int m, uint32_t (&w)[8]) {
+            const uint4 x = *reinterpret_cast<const uint4*>(vb + m * 512);
+            decode4<FMT>(x.x, w[0], w[1]);
+            decode4<FMT>(x.y, w[2], w[3]);
+            decode4<FMT>(x.z, w[4], w[5]);
+            decode4<FMT>(x.w, w[6], w[7]);
+          },
+          [](int) { return true; });
+      __syncwarp();  // the stage is written again by the next round's copy
+    }
+    cp_async_wait<0>();
+    if (here >= to) pdl_launch_dependents();
+
+    // merge the warps' rows in shared memory, over the rings
+    st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
+    st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
+    __syncthreads();
+    float2* ml_s = reinterpret_cast<float2*>(smem);
+    float* o_s = reinterpret_cast<float*>(smem + S::O);
+    int* last_s = reinterpret_cast<int*>(smem + S::FLAG);
+    if (q == 0) ml_s[warp * ROWS + r] = make_float2(st.m, st.l);
+#pragma unroll
+    for (int n2 = 0; n2 < D / 8; ++n2)
+      *reinterpret_cast<float2*>(o_s + (warp * ROWS + r) * D + 8 * n2 + 2 * q) =
+          make_float2(st.o[n2][0] + st.o[n2][2], st.o[n2][1] + st.o[n2][3]);
+    __syncthreads();
+
+    constexpr int D4 = D / 4;
+    auto fold = [](float& M, float& L, float (&acc)[4], float2 ml, float4 ov) {
+      const float mn = fmaxf(M, ml.x);
+      const float a = exp2_approx(M - mn), e = exp2_approx(ml.x - mn);
+      L = L * a + ml.y * e;
+      acc[0] = acc[0] * a + ov.x * e;
+      acc[1] = acc[1] * a + ov.y * e;
+      acc[2] = acc[2] * a + ov.z * e;
+      acc[3] = acc[3] * a + ov.w * e;
+      M = mn;
     };
-    attend_tile<D, true>(
-        st, qf, cq / fk, -__log2f(fv), fv, lane,
-        [&](int j, int h, uint32_t (&w)[8]) {
-          const int row = 8 * (r >> 1) + 2 * j + (r & 1);
+    auto store = [&](int g, int d, float L, const float (&acc)[4]) {
+      const float inv = 1.f / L;
+      const int s = g / p.groups, head = kvh * p.groups + g % p.groups;
+      T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.seq + s) * p.os +
+               static_cast<int64_t>(head) * D + d;
+      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(acc[0] * inv, acc[1] * inv),
+                                                  pack2<DT>(acc[2] * inv, acc[3] * inv));
+    };
+    // the CTAs whose pieces the unit lies in
+    const int first_cta = static_cast<int>(unit_at / line.piece);
+    const int last_cta = static_cast<int>((unit_at + w_unit - 1) / line.piece);
+    for (int idx = threadIdx.x; idx < ROWS * D4; idx += THREADS) {
+      const int lr = idx / D4, d = (idx % D4) * 4, g = rb * ROWS + lr;
+      if (g >= p.rows) continue;
+      float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kp + tile_off<D>(row, 8 * h + 2 * q + e));
-            w[4 * e] = to_half(x.x, fk);
-            w[4 * e + 1] = to_half(x.y, fk);
-            w[4 * e + 2] = to_half(x.z, fk);
-            w[4 * e + 3] = to_half(x.w, fk);
-          }
-        },
-        [&](int m, uint32_t (&w)[8]) {
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            uint32_t x[4];
-            load_column_tokens<D>(vtile, 2 * m + e, lane, x);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) w[4 * e + i] = to_half(x[i], fv);
-          }
-        },
-        [&](int token) { return t * BLOCK + token <= qpos; });
-
-    if (p.seq == 1 && rb == 0) {  // the append of a decode step
-      T* to = reinterpret_cast<T*>(p.tail) + bh * 2 * BLOCK * D;
-      if (open < BLOCK - 1) {
-        for (int c = lane; c < 2 * C16; c += 32) {
-          const bool val = c >= C16;
-          const int cc = val ? c - C16 : c;
-          *(reinterpret_cast<uint4*>(to + ((val ? BLOCK : 0) + open) * D) + cc) =
-              *reinterpret_cast<const uint4*>((val ? vp : kp) + tile_off<D>(open, cc));
-        }
+      for (int w = 0; w < WARPS; ++w) {
+        const float2 ml = ml_s[w * ROWS + lr];
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key of this row in the warp's tiles
+        fold(M, L, acc, ml, *reinterpret_cast<const float4*>(o_s + (w * ROWS + lr) * D + d));
+      }
+      if (first_cta == last_cta) {
+        store(g, d, L, acc);
       } else {
-        const int64_t block = bh * p.num_blocks + t;
-        const float sk = encode_keys<DT, FMT, D>(p.kc + block * (BLOCK * D), lane, [&](int tok, int c) {
-          return *reinterpret_cast<const uint4*>(kp + tile_off<D>(tok, c));
-        });
-        const float sv = encode_values<DT, FMT, D>(p.vc + block * (BLOCK * D), lane, vtile, vm);
-        if (lane == 0) reinterpret_cast<float2*>(p.scales)[block] = make_float2(sk, sv);
+        const int64_t slot = (static_cast<int64_t>(cta) * 2 + (cta == first_cta)) * ROWS + lr;
+        if (d == 0) p.part_ml[slot] = make_float2(M, L);
+        *reinterpret_cast<float4*>(p.part_o + slot * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
       }
     }
-  }
-  pdl_launch_dependents();
-
-  // merge the warps' rows in shared memory, over the stages
-  st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
-  st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
-  __syncthreads();
-  float2* ml_s = reinterpret_cast<float2*>(smem);
-  float* o_s = reinterpret_cast<float*>(smem + S::O);
-  int* last_s = reinterpret_cast<int*>(smem + S::FLAG);
-  if (q == 0) ml_s[warp * ROWS + r] = make_float2(st.m, st.l);
-#pragma unroll
-  for (int n = 0; n < D / 8; ++n)
-    *reinterpret_cast<float2*>(o_s + (warp * ROWS + r) * D + 8 * n + 2 * q) =
-        make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
-  __syncthreads();
-
-  constexpr int D4 = D / 4;
-  auto fold = [](float& M, float& L, float (&acc)[4], float2 ml, float4 ov) {
-    const float mn = fmaxf(M, ml.x);
-    const float a = exp2_approx(M - mn), e = exp2_approx(ml.x - mn);
-    L = L * a + ml.y * e;
-    acc[0] = acc[0] * a + ov.x * e;
-    acc[1] = acc[1] * a + ov.y * e;
-    acc[2] = acc[2] * a + ov.z * e;
-    acc[3] = acc[3] * a + ov.w * e;
-    M = mn;
-  };
-  auto store = [&](int g, int d, float L, const float (&acc)[4]) {
-    const float inv = 1.f / L;
-    const int s = g / p.groups, head = kvh * p.groups + g % p.groups;
-    T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.seq + s) * p.os +
-             static_cast<int64_t>(head) * D + d;
-    *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(acc[0] * inv, acc[1] * inv),
-                                                pack2<DT>(acc[2] * inv, acc[3] * inv));
-  };
-  for (int idx = threadIdx.x; idx < ROWS * D4; idx += THREADS) {
-    const int lr = idx / D4, d = (idx % D4) * 4, g = rb * ROWS + lr;
-    if (g >= p.rows) continue;
-    float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-    for (int w = 0; w < WARPS; ++w) {
-      const float2 ml = ml_s[w * ROWS + lr];
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key of this row in the warp's tiles
-      fold(M, L, acc, ml, *reinterpret_cast<const float4*>(o_s + (w * ROWS + lr) * D + d));
+    if (first_cta == last_cta) {
+      __syncthreads();  // the rings are free again
+      continue;
     }
-    if (n_chunks == 1) {
+    __threadfence();
+    __syncthreads();
+    if (threadIdx.x == 0) *last_s = atomicAdd(p.counters + first_cta, 1) == last_cta - first_cta;
+    __syncthreads();
+    if (!*last_s) continue;
+    __threadfence();
+    for (int idx = threadIdx.x; idx < ROWS * D4; idx += THREADS) {
+      const int lr = idx / D4, d = (idx % D4) * 4, g = rb * ROWS + lr;
+      if (g >= p.rows) continue;
+      float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+      for (int c = first_cta; c <= last_cta; ++c) {
+        const int64_t slot = (static_cast<int64_t>(c) * 2 + (c == first_cta)) * ROWS + lr;
+        const float2 ml = __ldcg(p.part_ml + slot);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        fold(M, L, acc, ml, __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + d)));
+      }
       store(g, d, L, acc);
-    } else {
-      const int64_t slot = (static_cast<int64_t>(unit) * p.n_chunks + chunk) * ROWS + lr;
-      if (d == 0) p.part_ml[slot] = make_float2(M, L);
-      *reinterpret_cast<float4*>(p.part_o + slot * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
     }
+    if (threadIdx.x == 0) p.counters[first_cta] = 0;
   }
-  if (n_chunks == 1) return;
-
-  __threadfence();
-  __syncthreads();
-  if (threadIdx.x == 0) *last_s = atomicAdd(p.counters + unit, 1) == n_chunks - 1;
-  __syncthreads();
-  if (!*last_s) return;
-  __threadfence();
-  for (int idx = threadIdx.x; idx < ROWS * D4; idx += THREADS) {
-    const int lr = idx / D4, d = (idx % D4) * 4, g = rb * ROWS + lr;
-    if (g >= p.rows) continue;
-    float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-    for (int c = 0; c < n_chunks; ++c) {
-      const int64_t slot = (static_cast<int64_t>(unit) * p.n_chunks + c) * ROWS + lr;
-      const float2 ml = __ldcg(p.part_ml + slot);
-      if (ml.x == -INFINITY && ml.y == 0.f) continue;
-      fold(M, L, acc, ml, __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + d)));
-    }
-    store(g, d, L, acc);
-  }
-  if (threadIdx.x == 0) p.counters[unit] = 0;
 }
 
-// The arrival counters come first and in a fixed size (a split needs fewer than two units for every SM), so calls
-// of different shapes that follow one another on a stream can share one workspace.
+// The arrival counters come first, then two slots of rows for each CTA: one size for all shapes of a head_dim, so
+// calls that follow one another on a stream can share one workspace.
 constexpr int64_t COUNTERS = 4096;
+constexpr int MAX_CTAS = COUNTERS / sizeof(int);
 
-struct Plan {
-  int n_rb, n_chunks;
-  int64_t units;
-  size_t ml_bytes, o_bytes;
-  size_t bytes() const { return n_chunks > 1 ? COUNTERS + ml_bytes + o_bytes : 0; }
-};
-
-size_t round_up(size_t x, size_t a) { return (x + a - 1) / a * a; }
-
-// Chunks of the key axis: enough CTAs for two on every SM, each with CHUNK_TILES tiles or more. Never fewer for a
-// longer cache, so that a workspace sized for the capacity serves every position.
-Plan make_plan(int batch, int num_kv_heads, int rows, int max_kv, int head_dim, int sm_count) {
-  Plan pl{};
-  pl.n_rb = (rows + ROWS - 1) / ROWS;
-  pl.units = static_cast<int64_t>(batch) * num_kv_heads * pl.n_rb;
-  const int tiles = max_kv / BLOCK + 1;
-  const int64_t most = (tiles + CHUNK_TILES - 1) / CHUNK_TILES;
-  const int64_t want = (2 * static_cast<int64_t>(std::max(sm_count, 1)) + pl.units - 1) / pl.units;
-  pl.n_chunks = static_cast<int>(std::max<int64_t>(1, std::min(most, want)));
-  if (pl.units * static_cast<int64_t>(sizeof(int)) > COUNTERS) pl.n_chunks = 1;
-  const size_t slots = static_cast<size_t>(pl.units) * pl.n_chunks * ROWS;
-  pl.ml_bytes = round_up(slots * sizeof(float2), 256);
-  pl.o_bytes = slots * head_dim * sizeof(float);
-  return pl;
+int ctas_per_sm(int head_dim) { return head_dim == 64 ? 3 : 2; }
+int total_ctas(int head_dim, int sm_count) { return std::min(MAX_CTAS, ctas_per_sm(head_dim) * std::max(sm_count, 1)); }
+int64_t workspace_bytes_for(int head_dim, int sm_count) {
+  return COUNTERS + int64_t(total_ctas(head_dim, sm_count)) * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
 }
 
 template <int DT, int FMT, int D>
-int launch(const AttnParams& p, dim3 grid, cudaStream_t st) {
+int launch(const AttnParams& p, int ctas, cudaStream_t st) {
   auto kern = kv8_attention_kernel<DT, FMT, D>;
   static bool configured[64] = {};
   DeviceInfo dev;
@@ -521,12 +665,12 @@ int launch(const AttnParams& p, dim3 grid, cudaStream_t st) {
       return rc;
     configured[dev.device] = true;
   }
-  return launch_kernel(kern, grid, dim3(THREADS), Smem<D>::TOTAL, st, 1, "kv8_attention", p);
+  return launch_kernel(kern, dim3(ctas), dim3(THREADS), Smem<D>::TOTAL, st, 1, "kv8_attention", p);
 }
 
 template <int DT, int FMT>
-int launch(const AttnParams& p, int head_dim, dim3 grid, cudaStream_t st) {
-  return head_dim == 64 ? launch<DT, FMT, 64>(p, grid, st) : launch<DT, FMT, 128>(p, grid, st);
+int launch(const AttnParams& p, int head_dim, int ctas, cudaStream_t st) {
+  return head_dim == 64 ? launch<DT, FMT, 64>(p, ctas, st) : launch<DT, FMT, 128>(p, ctas, st);
 }
 
 }  // namespace kv8
@@ -539,10 +683,7 @@ extern "C" int64_t tk_kv8_attention_workspace(int batch, int num_heads, int num_
     return 0;
   DeviceInfo di;
   if (current_device_info(&di)) return -1;
-  const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
-  if (rows > INT32_MAX) return 0;
-  return static_cast<int64_t>(
-      kv8::make_plan(batch, num_kv_heads, static_cast<int>(rows), max_kv, head_dim, di.sm_count).bytes());
+  return kv8::workspace_bytes_for(head_dim, di.sm_count);
 }
 
 extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
@@ -580,15 +721,12 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
-  const int max_kv = start_pos_device ? static_cast<int>(std::min<int64_t>(capacity, INT32_MAX)) : start_pos + seq;
   if (rows > (int64_t(65535) / num_kv_heads) * ROWS)
     return fail_invalid("kv8_attention: too many query rows per kv head");
-  const Plan pl = make_plan(batch, num_kv_heads, static_cast<int>(rows), max_kv, head_dim, di.sm_count);
-  if (pl.bytes() > 0) {
-    if (!workspace || workspace_bytes < static_cast<int64_t>(pl.bytes()))
-      return fail_invalid("kv8_attention: workspace missing or smaller than tk_kv8_attention_workspace()");
-    if (!aligned16(workspace)) return fail_invalid("kv8_attention: workspace must be 16-byte aligned");
-  }
+  if (!workspace || workspace_bytes < workspace_bytes_for(head_dim, di.sm_count))
+    return fail_invalid("kv8_attention: workspace missing or smaller than tk_kv8_attention_workspace()");
+  if (!aligned16(workspace)) return fail_invalid("kv8_attention: workspace must be 16-byte aligned");
+  const int ctas = total_ctas(head_dim, di.sm_count);
   AttnParams p{};
   p.q = q;
   p.qs = q_tok_stride;
@@ -613,24 +751,21 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   p.start_pos = start_pos;
   p.start_dev = start_pos_device;
   p.start_step = start_pos_step;
-  p.n_rb = pl.n_rb;
-  p.n_chunks = pl.n_chunks;
+  p.n_rb = static_cast<int>((rows + ROWS - 1) / ROWS);
+  p.batch = batch;
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
-  if (pl.bytes() > 0) {
-    char* ws = static_cast<char*>(workspace);
-    p.counters = reinterpret_cast<int*>(ws);
-    p.part_ml = reinterpret_cast<float2*>(ws + COUNTERS);
-    p.part_o = reinterpret_cast<float*>(ws + COUNTERS + pl.ml_bytes);
-  }
-  const dim3 grid(pl.n_chunks, num_kv_heads * pl.n_rb, batch);
+  char* ws = static_cast<char*>(workspace);
+  p.counters = reinterpret_cast<int*>(ws);
+  p.part_ml = reinterpret_cast<float2*>(ws + COUNTERS);
+  p.part_o = reinterpret_cast<float*>(ws + COUNTERS + int64_t(ctas) * 2 * ROWS * sizeof(float2));
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (dtype == TK_F16)
-    rc = format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, head_dim, grid, st)
-                               : launch<TK_F16, TK_KV8_INT8>(p, head_dim, grid, st);
+    rc = format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, head_dim, ctas, st)
+                               : launch<TK_F16, TK_KV8_INT8>(p, head_dim, ctas, st);
   else
-    rc = format == TK_KV8_E4M3 ? launch<TK_BF16, TK_KV8_E4M3>(p, head_dim, grid, st)
-                               : launch<TK_BF16, TK_KV8_INT8>(p, head_dim, grid, st);
+    rc = format == TK_KV8_E4M3 ? launch<TK_BF16, TK_KV8_E4M3>(p, head_dim, ctas, st)
+                               : launch<TK_BF16, TK_KV8_INT8>(p, head_dim, ctas, st);
   if (rc || seq == 1) return rc;
   return append(c, k, k_tok_stride, v, v_tok_stride, cos_table, sin_table, table_rows, batch, seq, num_kv_heads,
                 head_dim, start_pos, start_pos_device, start_pos_step, dtype, st);
