@@ -17,14 +17,15 @@
 //     scale_v cancels between numerator and denominator.
 //
 // Division of the work: all units' tiles in one line (a 16-bit tile counts TAIL_WEIGHT), cut into equal pieces, one
-// for each CTA that fits on the GPU at once. So long and short sequences, few units and many, keep every SM busy to
-// the end. A piece covers parts of one or more units; a unit that lies in several pieces is merged by the last of
-// their CTAs to arrive (a counter, which it returns to zero), in the order of the pieces, so results do not depend on
-// the order of arrival. No CTA waits for another. With little work the pieces keep PIECE_MIN tiles and begin at units.
-// Every warp of a CTA copies its tiles ahead into a ring of its own in shared memory (cp.async); the warps' (m, l, O)
-// rows are merged there. For S = 1 the warp that holds the open block also appends the row, or encodes the block if
-// the row completes it (nothing in the launch reads that block from the cache); for S > 1 a second launch appends,
-// since other CTAs still read the tail.
+// for each warp that fits on the GPU at once. So long and short sequences, few units and many, keep every SM busy to
+// the end, and no warp waits for another. A piece covers parts of one or more units; a unit that lies in several
+// pieces is merged by the last warp to arrive (counters, which it returns to zero), in the order of the pieces, so
+// results do not depend on the order of arrival; above 16 pieces in two steps, the first over aligned groups of 16,
+// so that no warp reads hundreds of partial results. With little work the pieces keep PIECE_MIN tiles and begin at
+// units. A warp copies its tiles ahead into a ring of its own in shared memory (cp.async), and the first tiles of its
+// next unit before it hands in the last one. For S = 1 the warp that holds the open block also appends the row, or
+// encodes the block if the row completes it (nothing in the launch reads that block from the cache); for S > 1 a
+// second launch appends, since other warps still read the tail.
 #include <algorithm>
 #include <string>
 
@@ -38,8 +39,9 @@ namespace kv8 {
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int ROWS = 8;         // query rows of a unit
-constexpr int TAIL_WEIGHT = 3;  // tiles that one 16-bit tile takes as long as
-constexpr int PIECE_MIN = 16;   // weight of a piece when there is little work
+constexpr int TAIL_WEIGHT = 4;  // tiles that one 16-bit tile takes as long as
+constexpr int PIECE_MIN = 8;    // weight of a piece when there is little work
+constexpr int GROUP = 16;       // pieces that are merged in one step
 
 struct AttnParams {
   const void* q;
@@ -64,9 +66,9 @@ struct AttnParams {
   int start_step;
   int n_rb, batch;
   float scale_log2;
-  int* counters;   // [CTAs], zero between launches
-  float2* part_ml;  // [CTAs][2][ROWS]: the unit that goes on from the piece before, the one that the next goes on with
-  float* part_o;    // [CTAs][2][ROWS][D]
+  int* counters;    // [warps][3], zero between launches
+  float2* part_ml;  // [warps][2][ROWS]: the unit that goes on from the piece before, the one that the next goes on with
+  float2* part_o;   // [warps][2][D / 8][32 lanes]
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -176,40 +178,61 @@ __device__ __forceinline__ void attend_tile(Rows<D>& st, const uint32_t (&qf)[D 
 template <int D>
 struct Smem {
   static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int HALF = BLOCK * D;                       // a block's keys or values
-  static constexpr int RING = STAGES * 2 * HALF;               // of one warp
-  static constexpr int TAIL = WARPS * RING;                    // a 16-bit tile: keys, then values
-  static constexpr int FLAG = TAIL + 2 * BLOCK * D * 2;
-  static constexpr int TOTAL = FLAG + 16;
-  static constexpr int O = WARPS * ROWS * 8;                   // merge, over the rings: float2 [WARPS][ROWS], then
-  static_assert(O + WARPS * ROWS * D * 4 <= TAIL, "the merge must fit in the rings");  // float [WARPS][ROWS][D]
+  static constexpr int HALF = BLOCK * D;      // a block's keys or values
+  static constexpr int STAGE = 2 * HALF;      // a block, or the keys or the values of a 16-bit tile
+  static constexpr int RING = STAGES * STAGE;  // of one warp
+  static constexpr int TOTAL = WARPS * RING;
 };
 
-// The pieces: unit u of sequence b (of `per_b` units) has weight(b); prefix sums place it on the line. Uniform
-// positions need no sums.
-struct Line {
-  int64_t total;  // weight of all units
-  int64_t piece;  // weight of a CTA's piece
-  bool padded;    // units begin at pieces
-};
+__device__ __forceinline__ int tiles16(int start, int seq) { return (start % BLOCK + seq + BLOCK - 1) / BLOCK; }
 
-__device__ __forceinline__ int64_t unit_weight(int start, int seq, int64_t piece_min) {
-  const int n8 = start / BLOCK;
-  const int64_t w = n8 + static_cast<int64_t>(TAIL_WEIGHT) * ((start % BLOCK + seq + BLOCK - 1) / BLOCK);
-  return piece_min > 1 ? (w + piece_min - 1) / piece_min * piece_min : w;
+// What a unit weighs on the line; `step` > 1: rounded up to whole pieces.
+__device__ __forceinline__ int unit_weight(int start, int seq, int step) {
+  const int w = start / BLOCK + TAIL_WEIGHT * tiles16(start, seq);
+  return (w + step - 1) / step * step;
 }
 
-// A position that does not fit has no weight: its sequence is left as it is.
+// A position that does not fit gives -1 (no weight): its sequence is left as it is.
 __device__ __forceinline__ int position_of(const AttnParams& p, int b) {
   const int start = p.start_dev ? __ldcg(p.start_dev + static_cast<int64_t>(b) * p.start_step) : p.start_pos;
   const int64_t end = static_cast<int64_t>(start) + p.seq;
   return start < 0 || end > static_cast<int64_t>(p.num_blocks) * BLOCK || (p.cos_t && end > p.table_rows) ? -1 : start;
 }
 
+// A warp's part of one unit.
+struct Segment {
+  int b, kvh, rb, start;
+  int t16_lo, t16_hi, lo, hi;  // 16-bit tiles and blocks
+  int first, last;             // the warps whose pieces the unit lies in
+};
+
+// Merged rows of a unit in the accumulators' layout: row r, columns 8n + 2q + {0, 1}.
+template <int D>
+struct Merged {
+  float m, l;
+  float2 o[D / 8];
+  __device__ __forceinline__ void clear() {
+    m = -INFINITY, l = 0.f;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) o[n] = make_float2(0.f, 0.f);
+  }
+  __device__ __forceinline__ void fold(float2 ml, const float2 (&v)[D / 8]) {
+    const float mn = fmaxf(m, ml.x);
+    const float base = mn == -INFINITY ? 0.f : mn;  // nothing but rows without a key so far
+    const float a = exp2_approx(m - base), e = exp2_approx(ml.x - base);
+    l = l * a + ml.y * e;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n) {
+      o[n].x = o[n].x * a + v[n].x * e;
+      o[n].y = o[n].y * a + v[n].y * e;
+    }
+    m = mn;
+  }
+};
+
 template <int DT, int FMT, int D>
 __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ int64_t sum_s[2][WARPS];
   using S = Smem<D>;
   using T = typename Dt<DT>::T;
   constexpr int C16 = D / 8;
@@ -217,65 +240,55 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, q = lane & 3;
   const int per_b = p.num_kv_heads * p.n_rb;
-  const int cta = blockIdx.x, ctas = gridDim.x;
+  const int n_warps = gridDim.x * WARPS;
+  const int me = warp * gridDim.x + blockIdx.x;  // neighbouring pieces on different SMs
+  uint8_t* ring = smem + warp * S::RING;
+  const uint32_t ring_u = smem_u32(ring);
   pdl_wait();
 
-  // the line: its length exact and padded, then this CTA's piece
+  // the line: its length exact and padded, then this warp's piece (all warps do the same sums)
   const bool ragged = p.start_dev && p.start_step;
   const int common = ragged ? 0 : position_of(p, 0);
-  Line line;
-  {
-    int64_t exact = 0, padded = 0;
-    bool bad = false;
-    if (!ragged) {
-      bad = common < 0;
-      exact = bad ? 0 : unit_weight(common, p.seq, 1) * p.batch;
-      padded = bad ? 0 : unit_weight(common, p.seq, PIECE_MIN) * p.batch;
-    } else {
-      for (int b = threadIdx.x; b < p.batch; b += THREADS) {
-        const int s = position_of(p, b);
-        bad |= s < 0;
-        exact += s < 0 ? 0 : unit_weight(s, p.seq, 1);
-        padded += s < 0 ? 0 : unit_weight(s, p.seq, PIECE_MIN);
-      }
-#pragma unroll
-      for (int o = 16; o > 0; o >>= 1) {
-        exact += __shfl_xor_sync(0xffffffffu, exact, o);
-        padded += __shfl_xor_sync(0xffffffffu, padded, o);
-      }
-      if (lane == 0) sum_s[0][warp] = exact, sum_s[1][warp] = padded;
-      __syncthreads();
-      exact = padded = 0;
-#pragma unroll
-      for (int w = 0; w < WARPS; ++w) exact += sum_s[0][w], padded += sum_s[1][w];
+  int exact = 0, padded = 0;
+  bool bad = false;
+  if (!ragged) {
+    bad = common < 0;
+    exact = bad ? 0 : unit_weight(common, p.seq, 1) * p.batch;
+    padded = bad ? 0 : unit_weight(common, p.seq, PIECE_MIN) * p.batch;
+  } else {
+    for (int b = lane; b < p.batch; b += 32) {
+      const int s = position_of(p, b);
+      bad |= s < 0;
+      exact += s < 0 ? 0 : unit_weight(s, p.seq, 1);
+      padded += s < 0 ? 0 : unit_weight(s, p.seq, PIECE_MIN);
     }
-    if (bad && cta == 0) record_device_error(TK_DEVERR_POSITION);
-    exact *= per_b;
-    padded *= per_b;
-    line.padded = padded <= static_cast<int64_t>(ctas) * PIECE_MIN;
-    line.total = line.padded ? padded : exact;
-    line.piece = line.padded ? PIECE_MIN : (exact + ctas - 1) / ctas;
+    exact = __reduce_add_sync(0xffffffffu, exact);
+    padded = __reduce_add_sync(0xffffffffu, padded);
   }
-  const int64_t from = line.piece * cta, to = min(line.total, from + line.piece);
-  if (from >= to) return;
+  if (bad && me == 0) record_device_error(TK_DEVERR_POSITION);
+  exact *= per_b;
+  padded *= per_b;
+  const bool whole = padded <= n_warps * PIECE_MIN;
+  const int total = whole ? padded : exact;
+  const int piece = whole ? PIECE_MIN : (exact + n_warps - 1) / n_warps;
+  const int step = whole ? PIECE_MIN : 1;
+  if (static_cast<int64_t>(piece) * me >= total) return;
+  const int from = piece * me, to = min(total, from + piece);
 
   // the sequence that `from` lies in, and where it begins
-  int b = 0;
-  int64_t at = 0;  // the line position of sequence b's first unit
-  const int64_t pad = line.padded ? PIECE_MIN : 1;
+  int b = 0, at = 0;
   if (!ragged) {
-    const int64_t w = unit_weight(common, p.seq, pad) * per_b;
-    b = static_cast<int>(from / w);
+    const int w = unit_weight(common, p.seq, step) * per_b;
+    b = from / w;
     at = b * w;
   } else {
-    // a warp at a time over 32 sequences; all warps do the same
     for (int b0 = 0;; b0 += 32) {
       const int s = b0 + lane < p.batch ? position_of(p, b0 + lane) : -1;
-      const int64_t mine = s < 0 ? 0 : unit_weight(s, p.seq, pad) * per_b;
-      int64_t upto = mine;
+      const int mine = s < 0 ? 0 : unit_weight(s, p.seq, step) * per_b;
+      int upto = mine;
 #pragma unroll
       for (int o = 1; o < 32; o <<= 1) {
-        const int64_t v = __shfl_up_sync(0xffffffffu, upto, o);
+        const int v = __shfl_up_sync(0xffffffffu, upto, o);
         if (lane >= o) upto += v;
       }
       const uint32_t past = __ballot_sync(0xffffffffu, at + upto > from);
@@ -289,84 +302,75 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     }
   }
 
-  const uint32_t ring = smem_u32(smem) + warp * S::RING;
-  const uint8_t* ring_p = smem + warp * S::RING;
-  int64_t here = from;
-  while (here < to) {
-    const int start = ragged ? position_of(p, b) : common;
-    const int64_t w_unit = start < 0 ? 0 : unit_weight(start, p.seq, pad);
-    if (here >= at + w_unit * per_b) {  // on to the next sequence (one without a valid position has no weight)
-      at += w_unit * per_b;
+  int here = from;
+  auto next_segment = [&](Segment& g) {  // false: the piece is done
+    if (here >= to) return false;
+    int start, w;
+    for (;;) {
+      start = ragged ? position_of(p, b) : common;
+      w = start < 0 ? 0 : unit_weight(start, p.seq, step);
+      if (here < at + w * per_b) break;
+      at += w * per_b;  // a sequence without a valid position has no weight
       ++b;
-      continue;
     }
-    const int y = static_cast<int>((here - at) / w_unit);
-    const int64_t unit_at = at + y * w_unit;                       // line position of the unit
-    const int kvh = y / p.n_rb, rb = y % p.n_rb;
-    const int open = start % BLOCK, n8 = start / BLOCK, n16 = (open + p.seq + BLOCK - 1) / BLOCK;
-    const int64_t end = static_cast<int64_t>(start) + p.seq;
-    const int64_t lo_w = here - unit_at, hi_w = min(to - unit_at, w_unit);
-    here = unit_at + hi_w;
-    const int64_t tail_w = static_cast<int64_t>(TAIL_WEIGHT) * n16;
+    const int y = (here - at) / w, unit = at + y * w;
+    const int n8 = start / BLOCK, n16 = tiles16(start, p.seq), w16 = TAIL_WEIGHT * n16;
+    const int lo_w = here - unit, hi_w = min(to - unit, w);
+    here = unit + hi_w;
+    g.b = b;
+    g.kvh = y / p.n_rb;
+    g.rb = y % p.n_rb;
+    g.start = start;
     // 16-bit tiles whose first weight lies in the piece, then blocks
-    const int t16_lo = static_cast<int>(min(static_cast<int64_t>(n16), (lo_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT));
-    const int t16_hi = static_cast<int>(min(static_cast<int64_t>(n16), (hi_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT));
-    const int lo = static_cast<int>(min(static_cast<int64_t>(n8), max(lo_w - tail_w, int64_t(0))));
-    const int hi = static_cast<int>(min(static_cast<int64_t>(n8), max(hi_w - tail_w, int64_t(0))));
-    const int64_t bh = static_cast<int64_t>(b) * p.num_kv_heads + kvh;
-    const uint8_t* kc = p.kc + bh * p.num_blocks * S::HALF;
-    const uint8_t* vc = p.vc + bh * p.num_blocks * S::HALF;
-    const float2* scales = reinterpret_cast<const float2*>(p.scales) + bh * p.num_blocks;
+    g.t16_lo = min(n16, (lo_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT);
+    g.t16_hi = min(n16, (hi_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT);
+    g.lo = min(n8, max(lo_w - w16, 0));
+    g.hi = min(n8, max(hi_w - w16, 0));
+    g.first = unit / piece;
+    g.last = (unit + w - 1) / piece;
+    return true;
+  };
 
-    // this warp's blocks: in rounds of one for each warp, without warp 0 for as long as it has 16-bit tiles
-    const int skip = TAIL_WEIGHT * (t16_hi - t16_lo), n = hi - lo;
-    auto tile_of = [&](int i) {
-      return lo + (i < skip ? i * (WARPS - 1) + warp - 1 : skip * (WARPS - 1) + (i - skip) * WARPS + warp);
-    };
-    const int i0 = warp == 0 ? skip : 0;
-    int n_my = i0;
-    {
-      const int free_first = skip * (WARPS - 1);
-      if (n <= free_first) {
-        if (warp > 0) n_my = (n - (warp - 1) + WARPS - 2) / (WARPS - 1);
-      } else {
-        n_my = skip + max(0, (n - free_first - warp + WARPS - 1) / WARPS);
+  // slot j of a segment's ring: the keys and the values of its 16-bit tiles, then its blocks
+  auto issue = [&](const Segment& g, int j) {
+    const int64_t bh = static_cast<int64_t>(g.b) * p.num_kv_heads + g.kvh;
+    const uint32_t dst = ring_u + (j % S::STAGES) * S::STAGE;
+    const int n16 = 2 * (g.t16_hi - g.t16_lo), t = g.lo + j - n16;
+    if (j < n16) {
+      if (g.t16_lo + j / 2 == 0) {  // the rows that the tail holds
+        const T* src = reinterpret_cast<const T*>(p.tail) + (bh * 2 + (j & 1)) * (BLOCK * D);
+        const int rows = g.start % BLOCK;
+        for (int idx = lane; idx < rows * C16; idx += 32) {
+          const int row = idx / C16, c = idx % C16;
+          cp_async16(dst + tile_off<D>(row, c), src + row * D + c * 8);
+        }
       }
-      n_my = max(n_my, i0);
+    } else if (t < g.hi) {
+      const int64_t block = (bh * p.num_blocks + t) * S::HALF + lane * 16;
+#pragma unroll
+      for (int i = 0; i < S::HALF / 512; ++i) cp_async16(dst + lane * 16 + i * 512, p.kc + block + i * 512);
+#pragma unroll
+      for (int i = 0; i < S::HALF / 512; ++i) cp_async16(dst + S::HALF + lane * 16 + i * 512, p.vc + block + i * 512);
     }
-    const T* tail = reinterpret_cast<const T*>(p.tail) + bh * 2 * BLOCK * D;
-    uint8_t* ktile = smem + S::TAIL;
-    uint8_t* vtile = ktile + BLOCK * D * 2;
-
-    auto copy_tail = [&](int t) {  // the rows of 16-bit tile t that the tail holds
-      if (t > 0) return;
-#pragma unroll 4
-      for (int idx = lane; idx < open * C16; idx += 32) {
-        const int row = idx / C16, c = idx % C16;
-        cp_async16(smem_u32(ktile) + tile_off<D>(row, c), tail + row * D + c * 8);
-        cp_async16(smem_u32(vtile) + tile_off<D>(row, c), tail + (BLOCK + row) * D + c * 8);
-      }
-    };
-    auto issue = [&](int i) {  // this warp's i-th block into its ring
-      if (i < n_my) {
-        const int64_t t = tile_of(i);
-        const uint32_t dst = ring + ((i - i0) % S::STAGES) * (2 * S::HALF) + lane * 16;
-        const uint8_t* ks = kc + t * S::HALF + lane * 16;
-        const uint8_t* vs = vc + t * S::HALF + lane * 16;
-#pragma unroll
-        for (int j = 0; j < S::HALF / 512; ++j) cp_async16(dst + j * 512, ks + j * 512);
-#pragma unroll
-        for (int j = 0; j < S::HALF / 512; ++j) cp_async16(dst + S::HALF + j * 512, vs + j * 512);
-      }
-      cp_async_commit();
-    };
-    if (warp == 0 && t16_lo < t16_hi) copy_tail(t16_lo);
     cp_async_commit();
-#pragma unroll
-    for (int i = 0; i < S::STAGES - 1; ++i) issue(i0 + i);
+  };
+  auto load_scale = [&](const Segment& g, int t) {
+    const int64_t bh = static_cast<int64_t>(g.b) * p.num_kv_heads + g.kvh;
+    return t + lane < g.hi ? __ldcg(reinterpret_cast<const float2*>(p.scales) + bh * p.num_blocks + t + lane)
+                           : make_float2(0.f, 1.f);
+  };
 
+  Segment g;
+  bool more = next_segment(g);
+  if (!more) return;
+#pragma unroll
+  for (int j = 0; j < S::STAGES - 1; ++j) issue(g, j);
+  float2 sc = load_scale(g, g.lo);
+
+  while (more) {
+    const int64_t bh = static_cast<int64_t>(g.b) * p.num_kv_heads + g.kvh;
     // this lane's share of query row r: rotated, brought to the f16 range, split in two
-    const int gr = rb * ROWS + r;
+    const int gr = g.rb * ROWS + r;
     int qpos = -1;  // a padding row sees no key of the 16-bit tiles, and its zeros harm nothing in the others
     uint32_t qf[H * 4][4];
     float cq;
@@ -378,9 +382,9 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 #pragma unroll
         for (int i = 0; i < 16; ++i) f[h][i] = 0.f;
       if (gr < p.rows) {
-        const int s = gr / p.groups, head = kvh * p.groups + gr % p.groups;
-        qpos = start + s;
-        const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(b) * p.seq + s) * p.qs +
+        const int s = gr / p.groups, head = g.kvh * p.groups + gr % p.groups;
+        qpos = g.start + s;
+        const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(g.b) * p.seq + s) * p.qs +
                        static_cast<int64_t>(head) * D;
 #pragma unroll
         for (int h = 0; h < H; ++h)
@@ -426,36 +430,35 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     st.m = -INFINITY;
     st.l = 0.f;
 #pragma unroll
-    for (int n2 = 0; n2 < D / 8; ++n2)
+    for (int n = 0; n < D / 8; ++n)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[n2][i] = 0.f;
+      for (int i = 0; i < 4; ++i) st.o[n][i] = 0.f;
 
-    // the open block and the new rows: warp 0
-    for (int t = t16_lo; warp == 0 && t < t16_hi; ++t) {
-      if (t > t16_lo) {
-        __syncwarp();
-        copy_tail(t);
-      }
-      const int n_rows = min(BLOCK, static_cast<int>(end - static_cast<int64_t>(n8 + t) * BLOCK));
+    int j = 0;  // the slot that is read next; slots up to j + STAGES - 2 are on their way
+    const int open = g.start % BLOCK, n8 = g.start / BLOCK;
+    for (int t = g.t16_lo; t < g.t16_hi; ++t, j += 2) {  // the open block and the new rows
+      uint8_t* ktile = ring + (j % S::STAGES) * S::STAGE;
+      uint8_t* vtile = ring + ((j + 1) % S::STAGES) * S::STAGE;
+      const int n_rows = min(BLOCK, open + p.seq - t * BLOCK);
       const int row0 = t == 0 ? open : 0;  // the first row that the call brings
       for (int idx = lane; idx < (BLOCK - row0) * C16; idx += 32) {
         const int row = row0 + idx / C16, c = idx % C16;
         uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
         if (row < n_rows) {
-          const int64_t s = t * BLOCK + row - open, tok = static_cast<int64_t>(b) * p.seq + s;
+          const int64_t s = t * BLOCK + row - open, tok = static_cast<int64_t>(g.b) * p.seq + s;
           kx = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + tok * p.ks +
-                                                     static_cast<int64_t>(kvh) * D) + c);
+                                                     static_cast<int64_t>(g.kvh) * D) + c);
           vx = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + tok * p.vs +
-                                                     static_cast<int64_t>(kvh) * D) + c);
+                                                     static_cast<int64_t>(g.kvh) * D) + c);
           if (p.cos_t) {
-            const int64_t ang = (static_cast<int64_t>(start) + s) * (D / 2) + c * 4;
+            const int64_t ang = (static_cast<int64_t>(g.start) + s) * (D / 2) + c * 4;
             rope_chunk<DT>(kx, p.cos_t + ang, p.sin_t + ang);
           }
         }
         *reinterpret_cast<uint4*>(ktile + tile_off<D>(row, c)) = kx;
         *reinterpret_cast<uint4*>(vtile + tile_off<D>(row, c)) = vx;
       }
-      if (t == 0) cp_async_wait<S::STAGES - 1>();  // the tail's rows; the blocks behind them may still be on the way
+      cp_async_wait<S::STAGES - 3>();  // both slots
       __syncwarp();
       uint32_t km = 0, vm = 0;
       if (DT == TK_BF16 || open + p.seq == BLOCK) {
@@ -482,8 +485,8 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
       };
       attend_tile<D, true>(
           st, qf, cq / fk, -__log2f(fv), fv, lane,
-          [&](int j, int h, uint32_t (&w)[8]) {
-            const int row = 8 * (r >> 1) + 2 * j + (r & 1);
+          [&](int jj, int h, uint32_t (&w)[8]) {
+            const int row = 8 * (r >> 1) + 2 * jj + (r & 1);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint4 x = *reinterpret_cast<const uint4*>(ktile + tile_off<D>(row, 8 * h + 2 * q + e));
@@ -504,7 +507,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
           },
           [&](int token) { return (n8 + t) * BLOCK + token <= qpos; });
 
-      if (p.seq == 1 && rb == 0) {  // the append of a decode step
+      if (p.seq == 1 && g.rb == 0) {  // the append of a decode step
         T* to_row = reinterpret_cast<T*>(p.tail) + bh * 2 * BLOCK * D;
         if (open < BLOCK - 1) {
           for (int c = lane; c < 2 * C16; c += 32) {
@@ -522,28 +525,30 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
           if (lane == 0) reinterpret_cast<float2*>(p.scales)[block] = make_float2(sk, sv);
         }
       }
+      __syncwarp();  // both slots are written again
+      issue(g, j + S::STAGES - 1);
+      issue(g, j + S::STAGES);
     }
 
-    // complete blocks; lane i keeps the scales of the warp's i-th block of each 32
-    float ks_l = 0.f, lv_l = 0.f, iv_l = 0.f;
-    for (int i = i0; i < n_my; ++i) {
-      if (((i - i0) & 31) == 0 && i + lane < n_my) {
-        const float2 sc = __ldcg(scales + tile_of(i + lane));
-        ks_l = sc.x;
+    // complete blocks; lane i keeps the scales of the i-th block of each 32
+    float lv_l = 0.f, iv_l = 0.f;
+    for (int t = g.lo; t < g.hi; ++t, ++j) {
+      const int i = (t - g.lo) & 31;
+      if (i == 0) {
+        if (t > g.lo) sc = load_scale(g, t);
         lv_l = __log2f(sc.y);
         iv_l = 1.f / sc.y;
       }
-      issue(i + S::STAGES - 1);
+      issue(g, j + S::STAGES - 1);
       cp_async_wait<S::STAGES - 1>();
-      __syncwarp();  // every lane's copies of block i have landed
-      const uint8_t* kb = ring_p + ((i - i0) % S::STAGES) * (2 * S::HALF) + lane * 16;
+      __syncwarp();  // every lane's copies of the block have landed
+      const uint8_t* kb = ring + (j % S::STAGES) * S::STAGE + lane * 16;
       const uint8_t* vb = kb + S::HALF;
-      const int src = (i - i0) & 31;
       attend_tile<D, false>(
-          st, qf, cq * __shfl_sync(0xffffffffu, ks_l, src), __shfl_sync(0xffffffffu, lv_l, src),
-          __shfl_sync(0xffffffffu, iv_l, src), lane,
-          [&](int j, int h, uint32_t (&w)[8]) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kb + (j * H + h) * 512);
+          st, qf, cq * __shfl_sync(0xffffffffu, sc.x, i), __shfl_sync(0xffffffffu, lv_l, i),
+          __shfl_sync(0xffffffffu, iv_l, i), lane,
+          [&](int jj, int h, uint32_t (&w)[8]) {
+            const uint4 x = *reinterpret_cast<const uint4*>(kb + (jj * H + h) * 512);
             decode4<FMT>(x.x, w[0], w[1]);
             decode4<FMT>(x.y, w[2], w[3]);
             decode4<FMT>(x.z, w[4], w[5]);
@@ -557,100 +562,99 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
             decode4<FMT>(x.w, w[6], w[7]);
           },
           [](int) { return true; });
-      __syncwarp();  // the stage is written again by the next round's copy
+      __syncwarp();  // the slot is written again by the next round's copy
     }
-    cp_async_wait<0>();
-    if (here >= to) pdl_launch_dependents();
 
-    // merge the warps' rows in shared memory, over the rings
-    st.l += __shfl_xor_sync(0xffffffffu, st.l, 1);
-    st.l += __shfl_xor_sync(0xffffffffu, st.l, 2);
-    __syncthreads();
-    float2* ml_s = reinterpret_cast<float2*>(smem);
-    float* o_s = reinterpret_cast<float*>(smem + S::O);
-    int* last_s = reinterpret_cast<int*>(smem + S::FLAG);
-    if (q == 0) ml_s[warp * ROWS + r] = make_float2(st.m, st.l);
+    // the next unit's first copies, then this unit's rows
+    const Segment done = g;
+    more = next_segment(g);
+    if (more) {
 #pragma unroll
-    for (int n2 = 0; n2 < D / 8; ++n2)
-      *reinterpret_cast<float2*>(o_s + (warp * ROWS + r) * D + 8 * n2 + 2 * q) =
-          make_float2(st.o[n2][0] + st.o[n2][2], st.o[n2][1] + st.o[n2][3]);
-    __syncthreads();
+      for (int i = 0; i < S::STAGES - 1; ++i) issue(g, i);
+      sc = load_scale(g, g.lo);
+    } else {
+      pdl_launch_dependents();
+    }
 
-    constexpr int D4 = D / 4;
-    auto fold = [](float& M, float& L, float (&acc)[4], float2 ml, float4 ov) {
-      const float mn = fmaxf(M, ml.x);
-      const float a = exp2_approx(M - mn), e = exp2_approx(ml.x - mn);
-      L = L * a + ml.y * e;
-      acc[0] = acc[0] * a + ov.x * e;
-      acc[1] = acc[1] * a + ov.y * e;
-      acc[2] = acc[2] * a + ov.z * e;
-      acc[3] = acc[3] * a + ov.w * e;
-      M = mn;
-    };
-    auto store = [&](int g, int d, float L, const float (&acc)[4]) {
-      const float inv = 1.f / L;
-      const int s = g / p.groups, head = kvh * p.groups + g % p.groups;
-      T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b) * p.seq + s) * p.os +
-               static_cast<int64_t>(head) * D + d;
-      *reinterpret_cast<uint2*>(dst) = make_uint2(pack2<DT>(acc[0] * inv, acc[1] * inv),
-                                                  pack2<DT>(acc[2] * inv, acc[3] * inv));
-    };
-    // the CTAs whose pieces the unit lies in
-    const int first_cta = static_cast<int>(unit_at / line.piece);
-    const int last_cta = static_cast<int>((unit_at + w_unit - 1) / line.piece);
-    for (int idx = threadIdx.x; idx < ROWS * D4; idx += THREADS) {
-      const int lr = idx / D4, d = (idx % D4) * 4, g = rb * ROWS + lr;
-      if (g >= p.rows) continue;
-      float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
+    Merged<D> mg;
+    mg.m = st.m;
+    mg.l = st.l + __shfl_xor_sync(0xffffffffu, st.l, 1);
+    mg.l += __shfl_xor_sync(0xffffffffu, mg.l, 2);
 #pragma unroll
-      for (int w = 0; w < WARPS; ++w) {
-        const float2 ml = ml_s[w * ROWS + lr];
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key of this row in the warp's tiles
-        fold(M, L, acc, ml, *reinterpret_cast<const float4*>(o_s + (w * ROWS + lr) * D + d));
+    for (int n = 0; n < D / 8; ++n)
+      mg.o[n] = make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
+    auto put = [&](int w) {  // into the slot of warp w
+      const int64_t slot = 2 * static_cast<int64_t>(w) + (w == done.first);
+      if (q == 0) p.part_ml[slot * ROWS + r] = make_float2(mg.m, mg.l);
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) p.part_o[(slot * (D / 8) + n) * 32 + lane] = mg.o[n];
+    };
+    auto arrive = [&](int* counter, int count) {  // whether this warp is the last of `count`
+      int last = 0;
+      __syncwarp();
+      if (lane == 0) {
+        __threadfence();
+        last = atomicAdd(counter, 1) == count - 1;
+        if (last) *counter = 0;
+        __threadfence();
       }
-      if (first_cta == last_cta) {
-        store(g, d, L, acc);
-      } else {
-        const int64_t slot = (static_cast<int64_t>(cta) * 2 + (cta == first_cta)) * ROWS + lr;
-        if (d == 0) p.part_ml[slot] = make_float2(M, L);
-        *reinterpret_cast<float4*>(p.part_o + slot * D + d) = make_float4(acc[0], acc[1], acc[2], acc[3]);
+      last = __shfl_sync(0xffffffffu, last, 0);
+      __syncwarp();
+      return last != 0;
+    };
+    auto gather = [&](int count, auto warp_of) {  // slots of warp_of(0 .. count - 1), in this order
+      constexpr int AHEAD = D == 64 ? 4 : 2;
+      mg.clear();
+      for (int i0 = 0; i0 < count; i0 += AHEAD) {
+        float2 ml[AHEAD], v[AHEAD][D / 8];
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) {
+          const int w = warp_of(min(i0 + i, count - 1));
+          const int64_t slot = 2 * static_cast<int64_t>(w) + (w == done.first);
+          ml[i] = __ldcg(p.part_ml + slot * ROWS + r);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) v[i][n] = __ldcg(p.part_o + (slot * (D / 8) + n) * 32 + lane);
+        }
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i)
+          if (i0 + i < count) mg.fold(ml[i], v[i]);
+      }
+    };
+    if (done.first != done.last) {
+      const int g_lo = done.first / GROUP, g_hi = done.last / GROUP, mine = me / GROUP;
+      auto leader = [&](int grp) { return max(done.first, grp * GROUP); };  // the group's first warp has its slot
+      const int w_lo = leader(mine), n_in = min(done.last, mine * GROUP + GROUP - 1) - w_lo + 1;
+      put(me);
+      if (n_in > 1) {
+        if (!arrive(p.counters + 2 * w_lo + (w_lo == done.first), n_in)) continue;
+        gather(n_in, [&](int i) { return w_lo + i; });
+      }
+      if (g_lo != g_hi) {
+        if (n_in > 1) put(w_lo);
+        if (!arrive(p.counters + 2 * n_warps + done.first, g_hi - g_lo + 1)) continue;
+        gather(g_hi - g_lo + 1, [&](int i) { return leader(g_lo + i); });
       }
     }
-    if (first_cta == last_cta) {
-      __syncthreads();  // the rings are free again
-      continue;
+    const int row = done.rb * ROWS + r;
+    if (row < p.rows) {
+      const float inv = 1.f / mg.l;
+      const int s = row / p.groups, head = done.kvh * p.groups + row % p.groups;
+      T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(done.b) * p.seq + s) * p.os +
+               static_cast<int64_t>(head) * D + 2 * q;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n)
+        *reinterpret_cast<uint32_t*>(dst + 8 * n) = pack2<DT>(mg.o[n].x * inv, mg.o[n].y * inv);
     }
-    __threadfence();
-    __syncthreads();
-    if (threadIdx.x == 0) *last_s = atomicAdd(p.counters + first_cta, 1) == last_cta - first_cta;
-    __syncthreads();
-    if (!*last_s) continue;
-    __threadfence();
-    for (int idx = threadIdx.x; idx < ROWS * D4; idx += THREADS) {
-      const int lr = idx / D4, d = (idx % D4) * 4, g = rb * ROWS + lr;
-      if (g >= p.rows) continue;
-      float M = -INFINITY, L = 0.f, acc[4] = {0.f, 0.f, 0.f, 0.f};
-      for (int c = first_cta; c <= last_cta; ++c) {
-        const int64_t slot = (static_cast<int64_t>(c) * 2 + (c == first_cta)) * ROWS + lr;
-        const float2 ml = __ldcg(p.part_ml + slot);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        fold(M, L, acc, ml, __ldcg(reinterpret_cast<const float4*>(p.part_o + slot * D + d)));
-      }
-      store(g, d, L, acc);
-    }
-    if (threadIdx.x == 0) p.counters[first_cta] = 0;
   }
 }
 
-// The arrival counters come first, then two slots of rows for each CTA: one size for all shapes of a head_dim, so
+// The arrival counters come first, then two slots of rows for each warp: one size for all shapes of a head_dim, so
 // calls that follow one another on a stream can share one workspace.
-constexpr int64_t COUNTERS = 4096;
-constexpr int MAX_CTAS = COUNTERS / sizeof(int);
-
-int ctas_per_sm(int head_dim) { return head_dim == 64 ? 3 : 2; }
-int total_ctas(int head_dim, int sm_count) { return std::min(MAX_CTAS, ctas_per_sm(head_dim) * std::max(sm_count, 1)); }
+int total_ctas(int head_dim, int sm_count) { return (head_dim == 64 ? 3 : 2) * std::max(sm_count, 1); }
+int64_t counter_bytes(int ctas) { return (int64_t(ctas) * WARPS * 3 * sizeof(int) + 255) / 256 * 256; }
 int64_t workspace_bytes_for(int head_dim, int sm_count) {
-  return COUNTERS + int64_t(total_ctas(head_dim, sm_count)) * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
+  const int ctas = total_ctas(head_dim, sm_count);
+  return counter_bytes(ctas) + int64_t(ctas) * WARPS * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
 }
 
 template <int DT, int FMT, int D>
@@ -721,8 +725,10 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
-  if (rows > (int64_t(65535) / num_kv_heads) * ROWS)
-    return fail_invalid("kv8_attention: too many query rows per kv head");
+  // the line of tiles is counted in 32 bits
+  const int64_t units = int64_t(batch) * num_kv_heads * ((rows + ROWS - 1) / ROWS);
+  const int64_t longest = num_blocks + int64_t(TAIL_WEIGHT) * (seq / BLOCK + 2) + PIECE_MIN;
+  if (units > INT32_MAX / longest) return fail_invalid("kv8_attention: too many query rows for one call");
   if (!workspace || workspace_bytes < workspace_bytes_for(head_dim, di.sm_count))
     return fail_invalid("kv8_attention: workspace missing or smaller than tk_kv8_attention_workspace()");
   if (!aligned16(workspace)) return fail_invalid("kv8_attention: workspace must be 16-byte aligned");
@@ -756,8 +762,10 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
   char* ws = static_cast<char*>(workspace);
   p.counters = reinterpret_cast<int*>(ws);
-  p.part_ml = reinterpret_cast<float2*>(ws + COUNTERS);
-  p.part_o = reinterpret_cast<float*>(ws + COUNTERS + int64_t(ctas) * 2 * ROWS * sizeof(float2));
+  ws += counter_bytes(ctas);
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  ws += int64_t(ctas) * WARPS * 2 * ROWS * sizeof(float2);
+  p.part_o = reinterpret_cast<float2*>(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (dtype == TK_F16)
