@@ -410,7 +410,7 @@ def test_position_tensor_graph_and_shared_workspace():
     torch.cuda.synchronize()
     for a, b in zip(cache, twin):
         assert torch.equal(torch.nan_to_num(a.float(), nan=-1.0), torch.nan_to_num(b.float(), nan=-1.0))
-    assert int(ws[:3 * 4 * 444 * 4].view(torch.int32).abs().sum()) == 0  # 148 SMs x 3 x 4 warps x 3 counters
+    assert int(ws[:3 * 444 * 4].view(torch.int32).abs().sum()) == 0  # 148 SMs x 3 CTAs x 3 counters
 
 
 @pytest.mark.gpu

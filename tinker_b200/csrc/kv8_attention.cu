@@ -16,14 +16,15 @@
 //     denominator is sum w / scale_v. So O needs no pass per block, w stays in [0, 1], and the rounding of log2
 //     scale_v cancels between numerator and denominator.
 //
-// Division of the work: all units' tiles in one line (a 16-bit tile counts TAIL_WEIGHT), cut into equal pieces, one
-// for each warp that fits on the GPU at once. So long and short sequences, few units and many, keep every SM busy to
-// the end, and no warp waits for another. A piece covers parts of one or more units; a unit that lies in several
-// pieces is merged by the last warp to arrive (counters, which it returns to zero), in the order of the pieces, so
-// results do not depend on the order of arrival; above 16 pieces in two steps, the first over aligned groups of 16,
-// so that no warp reads hundreds of partial results. With little work the pieces keep PIECE_MIN tiles and begin at
-// units. A warp copies its tiles ahead into a ring of its own in shared memory (cp.async), and the first tiles of its
-// next unit before it hands in the last one. For S = 1 the warp that holds the open block also appends the row, or
+// Division of the work: all units' tiles in one line (beginning a unit counts UNIT_WEIGHT, a 16-bit tile TAIL_WEIGHT),
+// cut into equal pieces, one for each warp that fits on the GPU at once. So long and short sequences, few units and
+// many, keep every SM busy to the end, and no CTA waits for another. A piece covers parts of one or more units. The
+// parts of a unit that lie in one CTA are merged in shared memory when its warps are done; where a unit lies in
+// several CTAs, the last of them to arrive (counters, which it returns to zero) merges their parts in the order of the
+// pieces, so results do not depend on the order of arrival; above 16 CTAs in two steps, the first over aligned groups of
+// 16, so that no warp reads hundreds of parts. With little work a unit gets CTAs of its own, PIECE_MIN for each warp.
+// A warp copies its tiles ahead into a ring of its own in shared memory (cp.async), and the first tiles of its next
+// unit before it puts the last one's rows away. For S = 1 the warp that holds the open block also appends the row, or
 // encodes the block if the row completes it (nothing in the launch reads that block from the cache); for S > 1 a
 // second launch appends, since other warps still read the tail.
 #include <algorithm>
@@ -40,8 +41,9 @@ constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
 constexpr int ROWS = 8;         // query rows of a unit
 constexpr int TAIL_WEIGHT = 4;  // tiles that one 16-bit tile takes as long as
-constexpr int PIECE_MIN = 8;    // weight of a piece when there is little work
-constexpr int GROUP = 16;       // pieces that are merged in one step
+constexpr int UNIT_WEIGHT = 1;  // and beginning a unit
+constexpr int PIECE_MIN = 4;    // weight of a piece when there is little work
+constexpr int GROUP = 16;       // CTAs that are merged in one step
 
 struct AttnParams {
   const void* q;
@@ -66,9 +68,9 @@ struct AttnParams {
   int start_step;
   int n_rb, batch;
   float scale_log2;
-  int* counters;    // [warps][3], zero between launches
-  float2* part_ml;  // [warps][2][ROWS]: the unit that goes on from the piece before, the one that the next goes on with
-  float2* part_o;   // [warps][2][D / 8][32 lanes]
+  int* counters;    // [CTAs][3], zero between launches
+  float2* part_ml;  // [CTAs][2][ROWS]: the unit that goes on from the CTA before, the one that the next goes on with
+  float2* part_o;   // [CTAs][2][D / 8][32 lanes]
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -181,14 +183,18 @@ struct Smem {
   static constexpr int HALF = BLOCK * D;      // a block's keys or values
   static constexpr int STAGE = 2 * HALF;      // a block, or the keys or the values of a 16-bit tile
   static constexpr int RING = STAGES * STAGE;  // of one warp
-  static constexpr int TOTAL = WARPS * RING;
+  static constexpr int PART = ROWS * D * 4 + ROWS * 8;  // a warp's rows of a unit: O, then (m, l)
+  static constexpr int HEAD = WARPS * RING;   // parts of units that go on from the piece before, one for each warp
+  static constexpr int INFO = HEAD + WARPS * PART;
+  static constexpr int TOTAL = INFO + WARPS * 2 * 32;
+  static_assert(PART <= RING, "the other parts lie over the rings");
 };
 
 __device__ __forceinline__ int tiles16(int start, int seq) { return (start % BLOCK + seq + BLOCK - 1) / BLOCK; }
 
 // What a unit weighs on the line; `step` > 1: rounded up to whole pieces.
 __device__ __forceinline__ int unit_weight(int start, int seq, int step) {
-  const int w = start / BLOCK + TAIL_WEIGHT * tiles16(start, seq);
+  const int w = UNIT_WEIGHT + start / BLOCK + TAIL_WEIGHT * tiles16(start, seq);
   return (w + step - 1) / step * step;
 }
 
@@ -204,6 +210,10 @@ struct Segment {
   int b, kvh, rb, start;
   int t16_lo, t16_hi, lo, hi;  // 16-bit tiles and blocks
   int first, last;             // the warps whose pieces the unit lies in
+};
+
+struct PartInfo {  // what a warp left in shared memory
+  int valid, b, kvh, rb, first, last;
 };
 
 // Merged rows of a unit in the accumulators' layout: row r, columns 8n + 2q + {0, 1}.
@@ -241,7 +251,8 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   const int r = lane >> 2, q = lane & 3;
   const int per_b = p.num_kv_heads * p.n_rb;
   const int n_warps = gridDim.x * WARPS;
-  const int me = warp * gridDim.x + blockIdx.x;  // neighbouring pieces on different SMs
+  const int me = blockIdx.x * WARPS + warp;
+  PartInfo* info = reinterpret_cast<PartInfo*>(smem + S::INFO);  // [WARPS][2]
   uint8_t* ring = smem + warp * S::RING;
   const uint32_t ring_u = smem_u32(ring);
   pdl_wait();
@@ -254,13 +265,13 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   if (!ragged) {
     bad = common < 0;
     exact = bad ? 0 : unit_weight(common, p.seq, 1) * p.batch;
-    padded = bad ? 0 : unit_weight(common, p.seq, PIECE_MIN) * p.batch;
+    padded = bad ? 0 : unit_weight(common, p.seq, WARPS * PIECE_MIN) * p.batch;
   } else {
     for (int b = lane; b < p.batch; b += 32) {
       const int s = position_of(p, b);
       bad |= s < 0;
       exact += s < 0 ? 0 : unit_weight(s, p.seq, 1);
-      padded += s < 0 ? 0 : unit_weight(s, p.seq, PIECE_MIN);
+      padded += s < 0 ? 0 : unit_weight(s, p.seq, WARPS * PIECE_MIN);
     }
     exact = __reduce_add_sync(0xffffffffu, exact);
     padded = __reduce_add_sync(0xffffffffu, padded);
@@ -271,13 +282,15 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   const bool whole = padded <= n_warps * PIECE_MIN;
   const int total = whole ? padded : exact;
   const int piece = whole ? PIECE_MIN : (exact + n_warps - 1) / n_warps;
-  const int step = whole ? PIECE_MIN : 1;
-  if (static_cast<int64_t>(piece) * me >= total) return;
-  const int from = piece * me, to = min(total, from + piece);
+  const int step = whole ? WARPS * PIECE_MIN : 1;
+  if (static_cast<int64_t>(piece) * (blockIdx.x * WARPS) >= total) return;  // nothing for the whole CTA
+  const int from = static_cast<int>(min(static_cast<int64_t>(piece) * me, static_cast<int64_t>(total)));
+  const int to = static_cast<int>(min(static_cast<int64_t>(from) + piece, static_cast<int64_t>(total)));
 
   // the sequence that `from` lies in, and where it begins
   int b = 0, at = 0;
-  if (!ragged) {
+  if (from >= to) {
+  } else if (!ragged) {
     const int w = unit_weight(common, p.seq, step) * per_b;
     b = from / w;
     at = b * w;
@@ -315,8 +328,8 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     }
     const int y = (here - at) / w, unit = at + y * w;
     const int n8 = start / BLOCK, n16 = tiles16(start, p.seq), w16 = TAIL_WEIGHT * n16;
-    const int lo_w = here - unit, hi_w = min(to - unit, w);
-    here = unit + hi_w;
+    const int lo_w = max(here - unit - UNIT_WEIGHT, 0), hi_w = max(min(to - unit, w) - UNIT_WEIGHT, 0);
+    here = min(to, unit + w);
     g.b = b;
     g.kvh = y / p.n_rb;
     g.rb = y % p.n_rb;
@@ -362,17 +375,43 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 
   Segment g;
   bool more = next_segment(g);
-  if (!more) return;
+  float2 sc = make_float2(0.f, 1.f);
+  uint4 q_raw[H][2];  // this lane's share of query row r
+  auto begin = [&]() {  // what a unit needs first, all in flight at once
+#pragma unroll 1
+    for (int j = 0; j < S::STAGES - 1; ++j) issue(g, j);
+    sc = load_scale(g, g.lo);
+    const int gr = g.rb * ROWS + r, s = gr / p.groups, head = g.kvh * p.groups + gr % p.groups;
+    const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(g.b) * p.seq + s) * p.qs +
+                   static_cast<int64_t>(head) * D;
 #pragma unroll
-  for (int j = 0; j < S::STAGES - 1; ++j) issue(g, j);
-  float2 sc = load_scale(g, g.lo);
+    for (int h = 0; h < H; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        q_raw[h][e] = gr < p.rows ? __ldcg(reinterpret_cast<const uint4*>(row) + 8 * h + 2 * q + e)
+                                  : make_uint4(0, 0, 0, 0);
+  };
+  if (more) begin();
+  if (lane == 0) info[2 * warp].valid = info[2 * warp + 1].valid = 0;
+
+  auto store = [&](const Merged<D>& mg, int b_, int kvh_, int rb_) {
+    const int row = rb_ * ROWS + r;
+    if (row >= p.rows) return;
+    const float inv = 1.f / mg.l;
+    const int s = row / p.groups, head = kvh_ * p.groups + row % p.groups;
+    T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b_) * p.seq + s) * p.os +
+             static_cast<int64_t>(head) * D + 2 * q;
+#pragma unroll
+    for (int n = 0; n < D / 8; ++n)
+      *reinterpret_cast<uint32_t*>(dst + 8 * n) = pack2<DT>(mg.o[n].x * inv, mg.o[n].y * inv);
+  };
 
   while (more) {
     const int64_t bh = static_cast<int64_t>(g.b) * p.num_kv_heads + g.kvh;
-    // this lane's share of query row r: rotated, brought to the f16 range, split in two
+    // query rows: rotated, brought to the f16 range, split in two
     const int gr = g.rb * ROWS + r;
-    int qpos = -1;  // a padding row sees no key of the 16-bit tiles, and its zeros harm nothing in the others
-    uint32_t qf[H * 4][4];
+    const int qpos = gr < p.rows ? g.start + gr / p.groups : -1;  // a padding row sees no key of the 16-bit tiles, and
+    uint32_t qf[H * 4][4];                                        // its zeros harm nothing in the others
     float cq;
     {
       float f[H][16];
@@ -380,35 +419,23 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int i = 0; i < 16; ++i) f[h][i] = 0.f;
-      if (gr < p.rows) {
-        const int s = gr / p.groups, head = g.kvh * p.groups + gr % p.groups;
-        qpos = g.start + s;
-        const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(g.b) * p.seq + s) * p.qs +
-                       static_cast<int64_t>(head) * D;
-#pragma unroll
-        for (int h = 0; h < H; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) {
-            const int c = 8 * h + 2 * q + e;
-            const uint4 x = __ldcg(reinterpret_cast<const uint4*>(row) + c);
-            const uint32_t w[4] = {x.x, x.y, x.z, x.w};
-            float cc[4] = {1.f, 1.f, 1.f, 1.f}, ss[4] = {0.f, 0.f, 0.f, 0.f};
-            if (p.cos_t) {
-              const int64_t ang = static_cast<int64_t>(qpos) * (D / 2) + c * 4;
-              const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos_t + ang));
-              const float4 d = __ldg(reinterpret_cast<const float4*>(p.sin_t + ang));
-              cc[0] = a.x, cc[1] = a.y, cc[2] = a.z, cc[3] = a.w;
-              ss[0] = d.x, ss[1] = d.y, ss[2] = d.z, ss[3] = d.w;
-            }
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-              const float2 v = unpack2<DT>(w[i]);
-              f[h][8 * e + 2 * i] = v.x * cc[i] - v.y * ss[i];
-              f[h][8 * e + 2 * i + 1] = v.x * ss[i] + v.y * cc[i];
-            }
+        for (int e = 0; e < 2; ++e) {
+          const uint32_t w[4] = {q_raw[h][e].x, q_raw[h][e].y, q_raw[h][e].z, q_raw[h][e].w};
+          float cc[4] = {1.f, 1.f, 1.f, 1.f}, ss[4] = {0.f, 0.f, 0.f, 0.f};
+          if (p.cos_t && qpos >= 0) {
+            const int64_t ang = static_cast<int64_t>(qpos) * (D / 2) + (8 * h + 2 * q + e) * 4;
+            const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos_t + ang));
+            const float4 d = __ldg(reinterpret_cast<const float4*>(p.sin_t + ang));
+            cc[0] = a.x, cc[1] = a.y, cc[2] = a.z, cc[3] = a.w;
+            ss[0] = d.x, ss[1] = d.y, ss[2] = d.z, ss[3] = d.w;
           }
-      }
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float2 v = unpack2<DT>(w[i]);
+            f[h][8 * e + 2 * i] = v.x * cc[i] - v.y * ss[i];
+            f[h][8 * e + 2 * i + 1] = v.x * ss[i] + v.y * cc[i];
+          }
+        }
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
@@ -436,11 +463,13 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 
     int j = 0;  // the slot that is read next; slots up to j + STAGES - 2 are on their way
     const int open = g.start % BLOCK, n8 = g.start / BLOCK;
+#pragma unroll 1
     for (int t = g.t16_lo; t < g.t16_hi; ++t, j += 2) {  // the open block and the new rows
       uint8_t* ktile = ring + (j % S::STAGES) * S::STAGE;
       uint8_t* vtile = ring + ((j + 1) % S::STAGES) * S::STAGE;
       const int n_rows = min(BLOCK, open + p.seq - t * BLOCK);
       const int row0 = t == 0 ? open : 0;  // the first row that the call brings
+#pragma unroll 1
       for (int idx = lane; idx < (BLOCK - row0) * C16; idx += 32) {
         const int row = row0 + idx / C16, c = idx % C16;
         uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
@@ -526,12 +555,13 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
         }
       }
       __syncwarp();  // both slots are written again
-      issue(g, j + S::STAGES - 1);
-      issue(g, j + S::STAGES);
+#pragma unroll 1
+      for (int i = S::STAGES - 1; i <= S::STAGES; ++i) issue(g, j + i);
     }
 
     // complete blocks; lane i keeps the scales of the i-th block of each 32
     float lv_l = 0.f, iv_l = 0.f;
+#pragma unroll 1
     for (int t = g.lo; t < g.hi; ++t, ++j) {
       const int i = (t - g.lo) & 31;
       if (i == 0) {
@@ -568,13 +598,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     // the next unit's first copies, then this unit's rows
     const Segment done = g;
     more = next_segment(g);
-    if (more) {
-#pragma unroll
-      for (int i = 0; i < S::STAGES - 1; ++i) issue(g, i);
-      sc = load_scale(g, g.lo);
-    } else {
-      pdl_launch_dependents();
-    }
+    if (more) begin();
 
     Merged<D> mg;
     mg.m = st.m;
@@ -583,78 +607,103 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 #pragma unroll
     for (int n = 0; n < D / 8; ++n)
       mg.o[n] = make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
-    auto put = [&](int w) {  // into the slot of warp w
-      const int64_t slot = 2 * static_cast<int64_t>(w) + (w == done.first);
-      if (q == 0) p.part_ml[slot * ROWS + r] = make_float2(mg.m, mg.l);
+    if (done.first == done.last) {
+      store(mg, done.b, done.kvh, done.rb);
+    } else {
+      // a unit that goes on from the piece before is this warp's first; any other is its last, when the ring is free
+      const int k = me == done.first;
+      uint8_t* part = k ? ring : smem + S::HEAD + warp * S::PART;
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) p.part_o[(slot * (D / 8) + n) * 32 + lane] = mg.o[n];
-    };
-    auto arrive = [&](int* counter, int count) {  // whether this warp is the last of `count`
-      int last = 0;
-      __syncwarp();
-      if (lane == 0) {
-        __threadfence();
-        last = atomicAdd(counter, 1) == count - 1;
-        if (last) *counter = 0;
-        __threadfence();
-      }
-      last = __shfl_sync(0xffffffffu, last, 0);
-      __syncwarp();
-      return last != 0;
-    };
-    auto gather = [&](int count, auto warp_of) {  // slots of warp_of(0 .. count - 1), in this order
-      constexpr int AHEAD = D == 64 ? 4 : 2;
-      mg.clear();
-      for (int i0 = 0; i0 < count; i0 += AHEAD) {
-        float2 ml[AHEAD], v[AHEAD][D / 8];
+      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(part + (n * 32 + lane) * 8) = mg.o[n];
+      if (q == 0) *reinterpret_cast<float2*>(part + ROWS * D * 4 + r * 8) = make_float2(mg.m, mg.l);
+      if (lane == 0) info[2 * warp + k] = PartInfo{1, done.b, done.kvh, done.rb, done.first, done.last};
+    }
+  }
+  pdl_launch_dependents();
+  __syncthreads();
+
+  // the parts of a unit in this CTA: merged by the warp that has the first of them
+  const int cta = blockIdx.x;
+#pragma unroll 1
+  for (int k = 0; k < 2; ++k) {
+    const PartInfo u = info[2 * warp + k];
+    if (!u.valid || (k == 0 && warp > 0)) continue;
+    Merged<D> mg;
+    mg.clear();
+    for (int w = warp; w < WARPS; ++w) {
+      const int kk = w == warp ? k : 0;
+      if (w > warp && !(blockIdx.x * WARPS + w <= u.last)) break;
+      const uint8_t* part = kk ? smem + w * S::RING : smem + S::HEAD + w * S::PART;
+      float2 v[D / 8];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) {
-          const int w = warp_of(min(i0 + i, count - 1));
-          const int64_t slot = 2 * static_cast<int64_t>(w) + (w == done.first);
-          ml[i] = __ldcg(p.part_ml + slot * ROWS + r);
+      for (int n = 0; n < D / 8; ++n) v[n] = *reinterpret_cast<const float2*>(part + (n * 32 + lane) * 8);
+      mg.fold(*reinterpret_cast<const float2*>(part + ROWS * D * 4 + r * 8), v);
+    }
+    const int c_first = u.first / WARPS, c_last = u.last / WARPS;
+    if (c_first != c_last) {
+      auto slot_of = [&](int c) { return 2 * static_cast<int64_t>(c) + (c == c_first); };
+      auto put = [&](int c) {
+        const int64_t slot = slot_of(c);
+        if (q == 0) p.part_ml[slot * ROWS + r] = make_float2(mg.m, mg.l);
 #pragma unroll
-          for (int n = 0; n < D / 8; ++n) v[i][n] = __ldcg(p.part_o + (slot * (D / 8) + n) * 32 + lane);
+        for (int n = 0; n < D / 8; ++n) p.part_o[(slot * (D / 8) + n) * 32 + lane] = mg.o[n];
+      };
+      auto arrive = [&](int* counter, int count) {  // whether this warp is the last of `count`
+        int last = 0;
+        __syncwarp();
+        if (lane == 0) {
+          __threadfence();
+          last = atomicAdd(counter, 1) == count - 1;
+          if (last) *counter = 0;
+          __threadfence();
         }
+        last = __shfl_sync(0xffffffffu, last, 0);
+        __syncwarp();
+        return last != 0;
+      };
+      auto gather = [&](int count, auto cta_of) {  // parts of CTAs cta_of(0 .. count - 1), in this order
+        constexpr int AHEAD = D == 64 ? 4 : 2;
+        mg.clear();
+#pragma unroll 1
+        for (int i0 = 0; i0 < count; i0 += AHEAD) {
+          float2 ml[AHEAD], v[AHEAD][D / 8];
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i)
-          if (i0 + i < count) mg.fold(ml[i], v[i]);
-      }
-    };
-    if (done.first != done.last) {
-      const int g_lo = done.first / GROUP, g_hi = done.last / GROUP, mine = me / GROUP;
-      auto leader = [&](int grp) { return max(done.first, grp * GROUP); };  // the group's first warp has its slot
-      const int w_lo = leader(mine), n_in = min(done.last, mine * GROUP + GROUP - 1) - w_lo + 1;
-      put(me);
+          for (int i = 0; i < AHEAD; ++i) {
+            const int64_t slot = slot_of(cta_of(min(i0 + i, count - 1)));
+            ml[i] = __ldcg(p.part_ml + slot * ROWS + r);
+#pragma unroll
+            for (int n = 0; n < D / 8; ++n) v[i][n] = __ldcg(p.part_o + (slot * (D / 8) + n) * 32 + lane);
+          }
+#pragma unroll
+          for (int i = 0; i < AHEAD; ++i)
+            if (i0 + i < count) mg.fold(ml[i], v[i]);
+        }
+      };
+      const int g_lo = c_first / GROUP, g_hi = c_last / GROUP, mine = cta / GROUP;
+      auto leader = [&](int grp) { return max(c_first, grp * GROUP); };  // the group's parts end up in its slot
+      const int c_lo = leader(mine), n_in = min(c_last, mine * GROUP + GROUP - 1) - c_lo + 1;
+      put(cta);
       if (n_in > 1) {
-        if (!arrive(p.counters + 2 * w_lo + (w_lo == done.first), n_in)) continue;
-        gather(n_in, [&](int i) { return w_lo + i; });
+        if (!arrive(p.counters + slot_of(c_lo), n_in)) continue;
+        gather(n_in, [&](int i) { return c_lo + i; });
       }
       if (g_lo != g_hi) {
-        if (n_in > 1) put(w_lo);
-        if (!arrive(p.counters + 2 * n_warps + done.first, g_hi - g_lo + 1)) continue;
+        if (n_in > 1) put(c_lo);
+        if (!arrive(p.counters + 2 * gridDim.x + c_first, g_hi - g_lo + 1)) continue;
         gather(g_hi - g_lo + 1, [&](int i) { return leader(g_lo + i); });
       }
     }
-    const int row = done.rb * ROWS + r;
-    if (row < p.rows) {
-      const float inv = 1.f / mg.l;
-      const int s = row / p.groups, head = done.kvh * p.groups + row % p.groups;
-      T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(done.b) * p.seq + s) * p.os +
-               static_cast<int64_t>(head) * D + 2 * q;
-#pragma unroll
-      for (int n = 0; n < D / 8; ++n)
-        *reinterpret_cast<uint32_t*>(dst + 8 * n) = pack2<DT>(mg.o[n].x * inv, mg.o[n].y * inv);
-    }
+    store(mg, u.b, u.kvh, u.rb);
   }
 }
 
-// The arrival counters come first, then two slots of rows for each warp: one size for all shapes of a head_dim, so
+// The arrival counters come first, then two slots of rows for each CTA: one size for all shapes of a head_dim, so
 // calls that follow one another on a stream can share one workspace.
 int total_ctas(int head_dim, int sm_count) { return (head_dim == 64 ? 3 : 2) * std::max(sm_count, 1); }
-int64_t counter_bytes(int ctas) { return (int64_t(ctas) * WARPS * 3 * sizeof(int) + 255) / 256 * 256; }
+int64_t counter_bytes(int ctas) { return (int64_t(ctas) * 3 * sizeof(int) + 255) / 256 * 256; }
 int64_t workspace_bytes_for(int head_dim, int sm_count) {
   const int ctas = total_ctas(head_dim, sm_count);
-  return counter_bytes(ctas) + int64_t(ctas) * WARPS * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
+  return counter_bytes(ctas) + int64_t(ctas) * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
 }
 
 template <int DT, int FMT, int D>
@@ -727,7 +776,7 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
   // the line of tiles is counted in 32 bits
   const int64_t units = int64_t(batch) * num_kv_heads * ((rows + ROWS - 1) / ROWS);
-  const int64_t longest = num_blocks + int64_t(TAIL_WEIGHT) * (seq / BLOCK + 2) + PIECE_MIN;
+  const int64_t longest = UNIT_WEIGHT + num_blocks + int64_t(TAIL_WEIGHT) * (seq / BLOCK + 2) + WARPS * PIECE_MIN;
   if (units > INT32_MAX / longest) return fail_invalid("kv8_attention: too many query rows for one call");
   if (!workspace || workspace_bytes < workspace_bytes_for(head_dim, di.sm_count))
     return fail_invalid("kv8_attention: workspace missing or smaller than tk_kv8_attention_workspace()");
@@ -764,7 +813,7 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   p.counters = reinterpret_cast<int*>(ws);
   ws += counter_bytes(ctas);
   p.part_ml = reinterpret_cast<float2*>(ws);
-  ws += int64_t(ctas) * WARPS * 2 * ROWS * sizeof(float2);
+  ws += int64_t(ctas) * 2 * ROWS * sizeof(float2);
   p.part_o = reinterpret_cast<float2*>(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
