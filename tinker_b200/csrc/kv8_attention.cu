@@ -29,6 +29,7 @@
 // second launch appends, since other warps still read the tail.
 #include <algorithm>
 #include <string>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "kv8_host.h"
@@ -67,6 +68,7 @@ struct AttnParams {
   const int* start_dev;
   int start_step;
   int n_rb, batch;
+  int most_ctas;  // CTAs that each unit can have for its own
   float scale_log2;
   int* counters;    // [CTAs][3], zero between launches
   float2* part_ml;  // [CTAs][2][ROWS]: the unit that goes on from the CTA before, the one that the next goes on with
@@ -114,34 +116,42 @@ struct Rows {
   float o[D / 8][4];
 };
 
-// One tile: K(j, h, w) and V(m, w) give code words (w = 0..7: f16 pairs of the lane's fragment, kv8.cuh), `sk` the
-// factor of the raw products, `lsv` = log2 of the values' scale, `isv` its inverse, allowed(token) the mask.
-template <int D, bool MASK, typename KF, typename VF, typename AF>
-__device__ __forceinline__ void attend_tile(Rows<D>& st, const uint32_t (&qf)[D / 64 * 4][4], float sk, float lsv,
-                                            float isv, int lane, KF key_words, VF value_words, AF allowed) {
+// N tiles in one step (independent products and one maximum, so that a warp that has a scheduler to itself waits
+// less): key_words(u, j, h, w) and value_words(u, m, w) give the f16 pairs w[0..7] of the lane's fragment of tile u
+// (kv8.cuh), `sk` the factor of the raw products, `lsv` log2 of the values' scale, `isv` its inverse, allowed(token)
+// the mask.
+template <int D, int N, bool MASK, typename KF, typename VF, typename AF>
+__device__ __forceinline__ void attend_tiles(Rows<D>& st, const uint32_t (&qf)[D / 64 * 4][4], const float (&sk)[N],
+                                             const float (&lsv)[N], const float (&isv)[N], int lane, KF key_words,
+                                             VF value_words, AF allowed) {
   constexpr int H = D / 64;
   const int q = lane & 3;
-  float s[4][2];
+  float s[N][4][2];
+  float mx = -INFINITY;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    float c[4] = {0.f, 0.f, 0.f, 0.f};
+  for (int u = 0; u < N; ++u)
 #pragma unroll
-    for (int h = 0; h < H; ++h) {
-      uint32_t w[8];
-      key_words(j, h, w);
+    for (int j = 0; j < 4; ++j) {
+      float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-      for (int t = 0; t < 4; ++t)
-        mma16816(c, qf[h * 4 + t][0], qf[h * 4 + t][1], qf[h * 4 + t][2], qf[h * 4 + t][3], w[2 * t], w[2 * t + 1]);
+      for (int h = 0; h < H; ++h) {
+        uint32_t w[8];
+        key_words(u, j, h, w);
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+          mma16816(c, qf[h * 4 + t][0], qf[h * 4 + t][1], qf[h * 4 + t][2], qf[h * 4 + t][3], w[2 * t], w[2 * t + 1]);
+      }
+      s[u][j][0] = fmaf(c[0] + c[2], sk[u], lsv[u]);
+      s[u][j][1] = fmaf(c[1] + c[3], sk[u], lsv[u]);
+      if (MASK) {
+        if (!allowed(8 * q + 2 * j)) s[u][j][0] = -INFINITY;
+        if (!allowed(8 * q + 2 * j + 1)) s[u][j][1] = -INFINITY;
+      }
     }
-    s[j][0] = fmaf(c[0] + c[2], sk, lsv);
-    s[j][1] = fmaf(c[1] + c[3], sk, lsv);
-    if (MASK) {
-      if (!allowed(8 * q + 2 * j)) s[j][0] = -INFINITY;
-      if (!allowed(8 * q + 2 * j + 1)) s[j][1] = -INFINITY;
-    }
-  }
-  float mx = fmaxf(fmaxf(fmaxf(s[0][0], s[0][1]), fmaxf(s[1][0], s[1][1])),
-                   fmaxf(fmaxf(s[2][0], s[2][1]), fmaxf(s[3][0], s[3][1])));
+#pragma unroll
+  for (int u = 0; u < N; ++u)
+#pragma unroll
+    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fmaxf(s[u][j][0], s[u][j][1]));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
   mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
   const float mn = fmaxf(st.m, mx);
@@ -155,31 +165,45 @@ __device__ __forceinline__ void attend_tile(Rows<D>& st, const uint32_t (&qf)[D 
     st.m = mn;
   }
   const float base = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet: all weights 0
-  uint32_t hi[4], lo[4];
-  float sum = 0.f;
 #pragma unroll
-  for (int j = 0; j < 4; ++j) {
-    const float w0 = exp2_approx(s[j][0] - base), w1 = exp2_approx(s[j][1] - base);
-    sum += w0 + w1;
-    split2(w0, w1, hi[j], lo[j]);
+  for (int u = 0; u < N; ++u) {
+    uint32_t hi[4], lo[4];
+    float sum = 0.f;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const float w0 = exp2_approx(s[u][j][0] - base), w1 = exp2_approx(s[u][j][1] - base);
+      sum += w0 + w1;
+      split2(w0, w1, hi[j], lo[j]);
+    }
+    st.l = fmaf(sum, isv[u], st.l);
+#pragma unroll
+    for (int m = 0; m < D / 16; ++m) {
+      uint32_t w[8];
+      value_words(u, m, w);
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+          mma16816(st.o[2 * m + e], hi[2 * i], lo[2 * i], hi[2 * i + 1], lo[2 * i + 1], w[4 * e + 2 * i],
+                   w[4 * e + 2 * i + 1]);
+    }
   }
-  st.l = fmaf(sum, isv, st.l);
-#pragma unroll
-  for (int m = 0; m < D / 16; ++m) {
-    uint32_t w[8];
-    value_words(m, w);
-#pragma unroll
-    for (int e = 0; e < 2; ++e)
-#pragma unroll
-      for (int i = 0; i < 2; ++i)
-        mma16816(st.o[2 * m + e], hi[2 * i], lo[2 * i], hi[2 * i + 1], lo[2 * i + 1], w[4 * e + 2 * i],
-                 w[4 * e + 2 * i + 1]);
-  }
+}
+
+// a / b for small non-negative numbers, without the latency of an integer division
+__device__ __forceinline__ int quotient(int a, int b) {
+  if (a >= 1 << 22) return a / b;
+  int x = static_cast<int>(__fdividef(static_cast<float>(a), static_cast<float>(b)));
+  const int rem = a - x * b;
+  return x + (rem >= b) - (rem < 0);
 }
 
 template <int D>
 struct Smem {
+  static constexpr int CTAS_SM = D == 64 ? 3 : 2;
+  static constexpr int SPLIT_COST = D == 64 ? 40 : 20;
   static constexpr int STAGES = D == 64 ? 4 : 3;
+  static constexpr int PAIR = D == 64 ? 2 : 1;                // blocks of a step
   static constexpr int HALF = BLOCK * D;      // a block's keys or values
   static constexpr int STAGE = 2 * HALF;      // a block, or the keys or the values of a 16-bit tile
   static constexpr int RING = STAGES * STAGE;  // of one warp
@@ -195,7 +219,7 @@ __device__ __forceinline__ int tiles16(int start, int seq) { return (start % BLO
 // What a unit weighs on the line; `step` > 1: rounded up to whole pieces.
 __device__ __forceinline__ int unit_weight(int start, int seq, int step) {
   const int w = UNIT_WEIGHT + start / BLOCK + TAIL_WEIGHT * tiles16(start, seq);
-  return (w + step - 1) / step * step;
+  return step == 1 ? w : quotient(w + step - 1, step) * step;
 }
 
 // A position that does not fit gives -1 (no weight): its sequence is left as it is.
@@ -240,8 +264,9 @@ struct Merged {
   }
 };
 
-template <int DT, int FMT, int D>
-__global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel(const AttnParams p) {
+// RAGGED: every sequence has a position of its own.
+template <int DT, int FMT, int D, bool RAGGED>
+__global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
   using S = Smem<D>;
   using T = typename Dt<DT>::T;
@@ -250,39 +275,52 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = lane >> 2, q = lane & 3;
   const int per_b = p.num_kv_heads * p.n_rb;
-  const int n_warps = gridDim.x * WARPS;
   const int me = blockIdx.x * WARPS + warp;
   PartInfo* info = reinterpret_cast<PartInfo*>(smem + S::INFO);  // [WARPS][2]
   uint8_t* ring = smem + warp * S::RING;
   const uint32_t ring_u = smem_u32(ring);
   pdl_wait();
 
-  // the line: its length exact and padded, then this warp's piece (all warps do the same sums)
-  const bool ragged = p.start_dev && p.start_step;
-  const int common = ragged ? 0 : position_of(p, 0);
-  int exact = 0, padded = 0;
+  // the line and this warp's piece (all warps do the same sums). `step` > 1: units are rounded up to whole CTAs
+  const int common = RAGGED ? 0 : position_of(p, 0);
+  const int n_units = p.batch * per_b, ctas = gridDim.x;
+  int total, piece, step;
   bool bad = false;
-  if (!ragged) {
+  if constexpr (!RAGGED) {
     bad = common < 0;
-    exact = bad ? 0 : unit_weight(common, p.seq, 1) * p.batch;
-    padded = bad ? 0 : unit_weight(common, p.seq, WARPS * PIECE_MIN) * p.batch;
+    const int w = bad ? 0 : unit_weight(common, p.seq, 1);
+    total = w * n_units;
+    piece = quotient(total + ctas * WARPS - 1, ctas * WARPS);
+    step = 1;
+    if (n_units <= ctas) {
+      // A unit in CTAs of its own is merged without leaving the SM; equal pieces balance better, but end with a merge
+      // through L2 that takes as long as SPLIT_COST weights on an SM. 64 sequences of 4 kv heads at 511 (256 units):
+      // 15.1 us in equal pieces, 10.1 us with a CTA for each unit; at 8184 52.0 and 55 us.
+      const int own = max(PIECE_MIN, quotient(w + p.most_ctas * WARPS - 1, p.most_ctas * WARPS));
+      const int per_unit = quotient(w + own * WARPS - 1, own * WARPS);
+      const int sms = ctas / Smem<D>::CTAS_SM;
+      if (quotient(n_units * per_unit + sms - 1, sms) * (own * WARPS) <= quotient(total, sms) + Smem<D>::SPLIT_COST) {
+        piece = own;
+        step = own * WARPS;
+        total = n_units * per_unit * step;
+      }
+    }
   } else {
+    int exact = 0, padded = 0;
     for (int b = lane; b < p.batch; b += 32) {
       const int s = position_of(p, b);
       bad |= s < 0;
       exact += s < 0 ? 0 : unit_weight(s, p.seq, 1);
       padded += s < 0 ? 0 : unit_weight(s, p.seq, WARPS * PIECE_MIN);
     }
-    exact = __reduce_add_sync(0xffffffffu, exact);
-    padded = __reduce_add_sync(0xffffffffu, padded);
+    exact = __reduce_add_sync(0xffffffffu, exact) * per_b;
+    padded = __reduce_add_sync(0xffffffffu, padded) * per_b;
+    const bool whole = padded <= ctas * WARPS * PIECE_MIN;
+    total = whole ? padded : exact;
+    piece = whole ? PIECE_MIN : (exact + ctas * WARPS - 1) / (ctas * WARPS);
+    step = whole ? WARPS * PIECE_MIN : 1;
   }
   if (bad && me == 0) record_device_error(TK_DEVERR_POSITION);
-  exact *= per_b;
-  padded *= per_b;
-  const bool whole = padded <= n_warps * PIECE_MIN;
-  const int total = whole ? padded : exact;
-  const int piece = whole ? PIECE_MIN : (exact + n_warps - 1) / n_warps;
-  const int step = whole ? WARPS * PIECE_MIN : 1;
   if (static_cast<int64_t>(piece) * (blockIdx.x * WARPS) >= total) return;  // nothing for the whole CTA
   const int from = static_cast<int>(min(static_cast<int64_t>(piece) * me, static_cast<int64_t>(total)));
   const int to = static_cast<int>(min(static_cast<int64_t>(from) + piece, static_cast<int64_t>(total)));
@@ -290,9 +328,9 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   // the sequence that `from` lies in, and where it begins
   int b = 0, at = 0;
   if (from >= to) {
-  } else if (!ragged) {
+  } else if constexpr (!RAGGED) {
     const int w = unit_weight(common, p.seq, step) * per_b;
-    b = from / w;
+    b = quotient(from, w);
     at = b * w;
   } else {
     for (int b0 = 0;; b0 += 32) {
@@ -315,32 +353,33 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     }
   }
 
+  auto token_of = [&](int row) { return p.seq == 1 ? 0 : quotient(row, p.groups); };
   int here = from;
   auto next_segment = [&](Segment& g) {  // false: the piece is done
     if (here >= to) return false;
     int start, w;
     for (;;) {
-      start = ragged ? position_of(p, b) : common;
+      start = RAGGED ? position_of(p, b) : common;
       w = start < 0 ? 0 : unit_weight(start, p.seq, step);
       if (here < at + w * per_b) break;
       at += w * per_b;  // a sequence without a valid position has no weight
       ++b;
     }
-    const int y = (here - at) / w, unit = at + y * w;
+    const int y = quotient(here - at, w), unit = at + y * w;
     const int n8 = start / BLOCK, n16 = tiles16(start, p.seq), w16 = TAIL_WEIGHT * n16;
     const int lo_w = max(here - unit - UNIT_WEIGHT, 0), hi_w = max(min(to - unit, w) - UNIT_WEIGHT, 0);
     here = min(to, unit + w);
     g.b = b;
-    g.kvh = y / p.n_rb;
-    g.rb = y % p.n_rb;
+    g.kvh = p.n_rb == 1 ? y : quotient(y, p.n_rb);
+    g.rb = y - g.kvh * p.n_rb;
     g.start = start;
     // 16-bit tiles whose first weight lies in the piece, then blocks
     g.t16_lo = min(n16, (lo_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT);
     g.t16_hi = min(n16, (hi_w + TAIL_WEIGHT - 1) / TAIL_WEIGHT);
     g.lo = min(n8, max(lo_w - w16, 0));
     g.hi = min(n8, max(hi_w - w16, 0));
-    g.first = unit / piece;
-    g.last = (unit + w - 1) / piece;
+    g.first = quotient(unit, piece);
+    g.last = quotient(unit + w - 1, piece);
     return true;
   };
 
@@ -350,13 +389,17 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     const uint32_t dst = ring_u + (j % S::STAGES) * S::STAGE;
     const int n16 = 2 * (g.t16_hi - g.t16_lo), t = g.lo + j - n16;
     if (j < n16) {
-      if (g.t16_lo + j / 2 == 0) {  // the rows that the tail holds
-        const T* src = reinterpret_cast<const T*>(p.tail) + (bh * 2 + (j & 1)) * (BLOCK * D);
-        const int rows = g.start % BLOCK;
-        for (int idx = lane; idx < rows * C16; idx += 32) {
-          const int row = idx / C16, c = idx % C16;
-          cp_async16(dst + tile_off<D>(row, c), src + row * D + c * 8);
-        }
+      // the open block's rows from the tail, the call's own (not rotated yet) from its tensors
+      const int open = g.start % BLOCK, row0 = (g.t16_lo + j / 2) * BLOCK - open;  // the call's row of the first token
+      const T* old = reinterpret_cast<const T*>(p.tail) + (bh * 2 + (j & 1)) * (BLOCK * D);
+      const int64_t stride = j & 1 ? p.vs : p.ks;
+      const T* fresh = reinterpret_cast<const T*>(j & 1 ? p.v : p.k) + static_cast<int64_t>(g.b) * p.seq * stride +
+                       static_cast<int64_t>(g.kvh) * D;
+      const int rows = min(BLOCK, p.seq - row0);
+#pragma unroll 1
+      for (int idx = lane; idx < rows * C16; idx += 32) {
+        const int row = idx / C16, c = idx % C16, s = row0 + row;
+        cp_async16(dst + tile_off<D>(row, c), (s < 0 ? old + row * D : fresh + s * stride) + c * 8);
       }
     } else if (t < g.hi) {
       const int64_t block = (bh * p.num_blocks + t) * S::HALF + lane * 16;
@@ -381,7 +424,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 #pragma unroll 1
     for (int j = 0; j < S::STAGES - 1; ++j) issue(g, j);
     sc = load_scale(g, g.lo);
-    const int gr = g.rb * ROWS + r, s = gr / p.groups, head = g.kvh * p.groups + gr % p.groups;
+    const int gr = g.rb * ROWS + r, s = token_of(gr), head = g.kvh * p.groups + gr - s * p.groups;
     const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(g.b) * p.seq + s) * p.qs +
                    static_cast<int64_t>(head) * D;
 #pragma unroll
@@ -398,7 +441,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     const int row = rb_ * ROWS + r;
     if (row >= p.rows) return;
     const float inv = 1.f / mg.l;
-    const int s = row / p.groups, head = kvh_ * p.groups + row % p.groups;
+    const int s = token_of(row), head = kvh_ * p.groups + row - s * p.groups;
     T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b_) * p.seq + s) * p.os +
              static_cast<int64_t>(head) * D + 2 * q;
 #pragma unroll
@@ -410,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
     const int64_t bh = static_cast<int64_t>(g.b) * p.num_kv_heads + g.kvh;
     // query rows: rotated, brought to the f16 range, split in two
     const int gr = g.rb * ROWS + r;
-    const int qpos = gr < p.rows ? g.start + gr / p.groups : -1;  // a padding row sees no key of the 16-bit tiles, and
+    const int qpos = gr < p.rows ? g.start + token_of(gr) : -1;  // a padding row sees no key of the 16-bit tiles, and
     uint32_t qf[H * 4][4];                                        // its zeros harm nothing in the others
     float cq;
     {
@@ -469,25 +512,20 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
       uint8_t* vtile = ring + ((j + 1) % S::STAGES) * S::STAGE;
       const int n_rows = min(BLOCK, open + p.seq - t * BLOCK);
       const int row0 = t == 0 ? open : 0;  // the first row that the call brings
-#pragma unroll 1
-      for (int idx = lane; idx < (BLOCK - row0) * C16; idx += 32) {
-        const int row = row0 + idx / C16, c = idx % C16;
-        uint4 kx = make_uint4(0, 0, 0, 0), vx = kx;
-        if (row < n_rows) {
-          const int64_t s = t * BLOCK + row - open, tok = static_cast<int64_t>(g.b) * p.seq + s;
-          kx = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.k) + tok * p.ks +
-                                                     static_cast<int64_t>(g.kvh) * D) + c);
-          vx = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const T*>(p.v) + tok * p.vs +
-                                                     static_cast<int64_t>(g.kvh) * D) + c);
-          if (p.cos_t) {
-            const int64_t ang = (static_cast<int64_t>(g.start) + s) * (D / 2) + c * 4;
-            rope_chunk<DT>(kx, p.cos_t + ang, p.sin_t + ang);
-          }
-        }
-        *reinterpret_cast<uint4*>(ktile + tile_off<D>(row, c)) = kx;
-        *reinterpret_cast<uint4*>(vtile + tile_off<D>(row, c)) = vx;
-      }
       cp_async_wait<S::STAGES - 3>();  // both slots
+      __syncwarp();
+#pragma unroll 1
+      for (int idx = row0 * C16 + lane; idx < BLOCK * C16; idx += 32) {  // rotate its keys, clear what is behind them
+        const int row = idx / C16, c = idx % C16;
+        uint4* kx = reinterpret_cast<uint4*>(ktile + tile_off<D>(row, c));
+        if (row >= n_rows) {
+          *kx = make_uint4(0, 0, 0, 0);
+          *reinterpret_cast<uint4*>(vtile + tile_off<D>(row, c)) = make_uint4(0, 0, 0, 0);
+        } else if (p.cos_t) {
+          const int64_t ang = (static_cast<int64_t>(n8 + t) * BLOCK + row) * (D / 2) + c * 4;
+          rope_chunk<DT>(*kx, p.cos_t + ang, p.sin_t + ang);
+        }
+      }
       __syncwarp();
       uint32_t km = 0, vm = 0;
       if (DT == TK_BF16 || open + p.seq == BLOCK) {
@@ -512,9 +550,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
           return h2_u32(__floats2half2_rn(v.x * f, v.y * f));
         }
       };
-      attend_tile<D, true>(
-          st, qf, cq / fk, -__log2f(fv), fv, lane,
-          [&](int jj, int h, uint32_t (&w)[8]) {
+      const float sk1[1] = {cq / fk}, lsv1[1] = {-__log2f(fv)}, isv1[1] = {fv};
+      attend_tiles<D, 1, true>(
+          st, qf, sk1, lsv1, isv1, lane,
+          [&](int, int jj, int h, uint32_t (&w)[8]) {
             const int row = 8 * (r >> 1) + 2 * jj + (r & 1);
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
@@ -525,7 +564,7 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
               w[4 * e + 3] = to_half(x.w, fk);
             }
           },
-          [&](int m, uint32_t (&w)[8]) {
+          [&](int, int m, uint32_t (&w)[8]) {
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               uint32_t x[4];
@@ -559,10 +598,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
       for (int i = S::STAGES - 1; i <= S::STAGES; ++i) issue(g, j + i);
     }
 
-    // complete blocks; lane i keeps the scales of the i-th block of each 32
+    // complete blocks, PAIR of them in a step; lane i keeps the scales of the i-th block of each 32
     float lv_l = 0.f, iv_l = 0.f;
-#pragma unroll 1
-    for (int t = g.lo; t < g.hi; ++t, ++j) {
+    auto blocks = [&](auto count, int t) {
+      constexpr int N = decltype(count)::value;
       const int i = (t - g.lo) & 31;
       if (i == 0) {
         if (t > g.lo) sc = load_scale(g, t);
@@ -570,30 +609,46 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
         iv_l = 1.f / sc.y;
       }
       issue(g, j + S::STAGES - 1);
-      cp_async_wait<S::STAGES - 1>();
-      __syncwarp();  // every lane's copies of the block have landed
-      const uint8_t* kb = ring + (j % S::STAGES) * S::STAGE + lane * 16;
-      const uint8_t* vb = kb + S::HALF;
-      attend_tile<D, false>(
-          st, qf, cq * __shfl_sync(0xffffffffu, sc.x, i), __shfl_sync(0xffffffffu, lv_l, i),
-          __shfl_sync(0xffffffffu, iv_l, i), lane,
-          [&](int jj, int h, uint32_t (&w)[8]) {
-            const uint4 x = *reinterpret_cast<const uint4*>(kb + (jj * H + h) * 512);
+      cp_async_wait<S::STAGES - N>();
+      __syncwarp();  // every lane's copies of the blocks have landed
+      float sk[N], lsv[N], isv[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u) {
+        sk[u] = cq * __shfl_sync(0xffffffffu, sc.x, i + u);
+        lsv[u] = __shfl_sync(0xffffffffu, lv_l, i + u);
+        isv[u] = __shfl_sync(0xffffffffu, iv_l, i + u);
+      }
+      const uint8_t* slot[N];
+#pragma unroll
+      for (int u = 0; u < N; ++u) slot[u] = ring + ((j + u) % S::STAGES) * S::STAGE + lane * 16;
+      attend_tiles<D, N, false>(
+          st, qf, sk, lsv, isv, lane,
+          [&](int u, int jj, int h, uint32_t (&w)[8]) {
+            const uint4 x = *reinterpret_cast<const uint4*>(slot[u] + (jj * H + h) * 512);
             decode4<FMT>(x.x, w[0], w[1]);
             decode4<FMT>(x.y, w[2], w[3]);
             decode4<FMT>(x.z, w[4], w[5]);
             decode4<FMT>(x.w, w[6], w[7]);
           },
-          [&](int m, uint32_t (&w)[8]) {
-            const uint4 x = *reinterpret_cast<const uint4*>(vb + m * 512);
+          [&](int u, int m, uint32_t (&w)[8]) {
+            const uint4 x = *reinterpret_cast<const uint4*>(slot[u] + S::HALF + m * 512);
             decode4<FMT>(x.x, w[0], w[1]);
             decode4<FMT>(x.y, w[2], w[3]);
             decode4<FMT>(x.z, w[4], w[5]);
             decode4<FMT>(x.w, w[6], w[7]);
           },
           [](int) { return true; });
-      __syncwarp();  // the slot is written again by the next round's copy
+      __syncwarp();  // the slots are written again by the next copies
+      if constexpr (N == 2) issue(g, j + S::STAGES);
+      j += N;
+    };
+    int t = g.lo;
+    if constexpr (S::PAIR == 2) {
+#pragma unroll 1
+      for (; t + 1 < g.hi; t += 2) blocks(std::integral_constant<int, 2>(), t);
     }
+#pragma unroll 1
+    for (; t < g.hi; ++t) blocks(std::integral_constant<int, 1>(), t);
 
     // the next unit's first copies, then this unit's rows
     const Segment done = g;
@@ -622,17 +677,23 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
   pdl_launch_dependents();
   __syncthreads();
 
-  // the parts of a unit in this CTA: merged by the warp that has the first of them
+  // the parts of a unit in this CTA: merged by the warp in which the unit begins; those of the unit that goes on from
+  // the CTA before by a warp in which none begins, if there is one
   const int cta = blockIdx.x;
+  int head_by = 0;
+#pragma unroll
+  for (int w = WARPS - 1; w >= 0; --w)
+    if (!info[2 * w + 1].valid) head_by = w;
 #pragma unroll 1
-  for (int k = 0; k < 2; ++k) {
-    const PartInfo u = info[2 * warp + k];
-    if (!u.valid || (k == 0 && warp > 0)) continue;
+  for (int k = 1; k >= 0; --k) {
+    const int w0 = k ? warp : 0;  // where the unit's parts begin
+    const PartInfo u = info[2 * w0 + k];
+    if (!u.valid || (k == 0 && warp != head_by)) continue;
     Merged<D> mg;
     mg.clear();
-    for (int w = warp; w < WARPS; ++w) {
-      const int kk = w == warp ? k : 0;
-      if (w > warp && !(blockIdx.x * WARPS + w <= u.last)) break;
+    for (int w = w0; w < WARPS; ++w) {
+      const int kk = w == w0 ? k : 0;
+      if (w > w0 && blockIdx.x * WARPS + w > u.last) break;
       const uint8_t* part = kk ? smem + w * S::RING : smem + S::HEAD + w * S::PART;
       float2 v[D / 8];
 #pragma unroll
@@ -654,8 +715,10 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
         if (lane == 0) {
           __threadfence();
           last = atomicAdd(counter, 1) == count - 1;
-          if (last) *counter = 0;
-          __threadfence();
+          if (last) {
+            *counter = 0;
+            __threadfence();
+          }
         }
         last = __shfl_sync(0xffffffffu, last, 0);
         __syncwarp();
@@ -699,16 +762,18 @@ __global__ void __launch_bounds__(THREADS, D == 64 ? 3 : 2) kv8_attention_kernel
 
 // The arrival counters come first, then two slots of rows for each CTA: one size for all shapes of a head_dim, so
 // calls that follow one another on a stream can share one workspace.
-int total_ctas(int head_dim, int sm_count) { return (head_dim == 64 ? 3 : 2) * std::max(sm_count, 1); }
+int total_ctas(int head_dim, int sm_count) {
+  return (head_dim == 64 ? Smem<64>::CTAS_SM : Smem<128>::CTAS_SM) * std::max(sm_count, 1);
+}
 int64_t counter_bytes(int ctas) { return (int64_t(ctas) * 3 * sizeof(int) + 255) / 256 * 256; }
 int64_t workspace_bytes_for(int head_dim, int sm_count) {
   const int ctas = total_ctas(head_dim, sm_count);
   return counter_bytes(ctas) + int64_t(ctas) * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
 }
 
-template <int DT, int FMT, int D>
+template <int DT, int FMT, int D, bool RAGGED>
 int launch(const AttnParams& p, int ctas, cudaStream_t st) {
-  auto kern = kv8_attention_kernel<DT, FMT, D>;
+  auto kern = kv8_attention_kernel<DT, FMT, D, RAGGED>;
   static bool configured[64] = {};
   DeviceInfo dev;
   if (int rc = current_device_info(&dev)) return rc;
@@ -723,7 +788,9 @@ int launch(const AttnParams& p, int ctas, cudaStream_t st) {
 
 template <int DT, int FMT>
 int launch(const AttnParams& p, int head_dim, int ctas, cudaStream_t st) {
-  return head_dim == 64 ? launch<DT, FMT, 64>(p, ctas, st) : launch<DT, FMT, 128>(p, ctas, st);
+  const bool ragged = p.start_dev && p.start_step;
+  if (head_dim == 64) return ragged ? launch<DT, FMT, 64, true>(p, ctas, st) : launch<DT, FMT, 64, false>(p, ctas, st);
+  return ragged ? launch<DT, FMT, 128, true>(p, ctas, st) : launch<DT, FMT, 128, false>(p, ctas, st);
 }
 
 }  // namespace kv8
@@ -808,6 +875,7 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   p.start_step = start_pos_step;
   p.n_rb = static_cast<int>((rows + ROWS - 1) / ROWS);
   p.batch = batch;
+  p.most_ctas = static_cast<int>(std::max<int64_t>(1, ctas / units));
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
   char* ws = static_cast<char*>(workspace);
   p.counters = reinterpret_cast<int*>(ws);
