@@ -410,7 +410,7 @@ def test_position_tensor_graph_and_shared_workspace():
     torch.cuda.synchronize()
     for a, b in zip(cache, twin):
         assert torch.equal(torch.nan_to_num(a.float(), nan=-1.0), torch.nan_to_num(b.float(), nan=-1.0))
-    assert int(ws[:3 * 444 * 4].view(torch.int32).abs().sum()) == 0  # 148 SMs x 3 CTAs x 3 counters
+    assert int(ws[:4 * 148 * 3 * 4].view(torch.int32).abs().sum()) == 0  # three counters for each CTA
 
 
 @pytest.mark.gpu

@@ -5,16 +5,20 @@
 // call's own rows in 16 bits. q is rotated in fp32 and not rounded, k is rotated and rounded to the model type (what
 // the cache keeps), o = softmax(q k^T / sqrt(D)) v, rounded once. Then the new rows are appended.
 //
-// Products: m16n8k16 with f16 operands and fp32 sums, a warp for each tile of 32 keys.
+// Products: m16n8k16 with f16 operands and fp32 sums, a warp for each tile of 32 keys, with the keys (and the columns
+// of V) as the 16 rows of the product and the query rows as its 8 columns:
 //   * codes are exact in f16, so are 16-bit rows times a power of two that brings the tile's largest magnitude to
 //     [2^14, 2^15) (bf16; its 8 bits stay whole for 28 binades below that);
-//   * the 8 query rows of a unit (one sequence, kv head and block of rows) fill rows 0-7 of the A operand with
-//     f16(q), rows 8-15 with the remainder q - f16(q), likewise the probabilities: nothing is lost to 16-bit operands,
-//     and the rows that GQA leaves unused are free;
+//   * a query row takes two columns, f16(q) and the remainder q - f16(q), likewise its probabilities, whose sum stays
+//     in one lane: nothing is lost to 16-bit operands. Four query rows fill the 8 columns, which is what GQA with up
+//     to four heads for each kv head needs; eight rows (NG = 2) take every product twice;
 //   * the scale of a block's values goes into the exponent: with x = s * scale_k / sqrt(D) * log2 e, a weight is
 //     w = 2^(x + log2 scale_v - m), m the running maximum of that sum, O = sum w * code, and the softmax's
 //     denominator is sum w / scale_v. So O needs no pass per block, w stays in [0, 1], and the rounding of log2
 //     scale_v cancels between numerator and denominator.
+// (The keys as columns, with f16(q) and remainder as two halves of the 16 rows, took 274 instead of some 170
+// instructions for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 17 us for 64
+// sequences of 4 kv heads at 2047.)
 //
 // Division of the work: all units' tiles in one line (beginning a unit counts UNIT_WEIGHT, a 16-bit tile TAIL_WEIGHT),
 // cut into equal pieces, one for each warp that fits on the GPU at once. So long and short sequences, few units and
@@ -40,10 +44,10 @@ namespace kv8 {
 
 constexpr int WARPS = 4;
 constexpr int THREADS = WARPS * 32;
-constexpr int ROWS = 8;         // query rows of a unit
 constexpr int TAIL_WEIGHT = 4;  // tiles that one 16-bit tile takes as long as
 constexpr int UNIT_WEIGHT = 1;  // and beginning a unit
 constexpr int PIECE_MIN = 4;    // weight of a piece when there is little work
+constexpr int MERGE_COST = 8;   // weight that a warp could take while the parts of two CTAs are merged
 constexpr int GROUP = 16;       // CTAs that are merged in one step
 
 struct AttnParams {
@@ -71,8 +75,9 @@ struct AttnParams {
   int most_ctas;  // CTAs that each unit can have for its own
   float scale_log2;
   int* counters;    // [CTAs][3], zero between launches
-  float2* part_ml;  // [CTAs][2][ROWS]: the unit that goes on from the CTA before, the one that the next goes on with
-  float2* part_o;   // [CTAs][2][D / 8][32 lanes]
+  // [CTAs][2: the unit that goes on from the CTA before, the one that the next goes on with][NG][...]
+  float2* part_ml;  // [4 rows]
+  float* part_o;    // [D / 8][32 lanes]
 };
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
@@ -108,84 +113,111 @@ __device__ __forceinline__ float to_f16_range(uint32_t amax_bits) {
   return __uint_as_float(static_cast<uint32_t>(min(254, 268 - e)) << 23);
 }
 
-// State of a warp's 8 query rows: lane 4r + q holds row r; m and l of that row (l: this lane's share), O columns
-// 8n + 2q + {0, 1} of it in o[n][0..1] and the part that comes from the probabilities' remainders in o[n][2..3].
-template <int D>
+// 8 x 8 16-bit matrix transposed: lane 4i + q gives row i, columns 2q and 2q + 1, and takes them of the transpose.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
+}
+
+// State of a warp's 4 NG query rows; lane 4r + q has row 4g + q, of that row m, and its own keys' share of l, and the
+// columns 16n + r and 16n + 8 + r of O as sums of two parts, o[g][n][0] + [1] and [2] + [3].
+template <int D, int NG>
 struct Rows {
-  float m, l;
-  float o[D / 8][4];
+  float m[NG], l[NG];
+  float o[NG][D / 16][4];
 };
 
 // N tiles in one step (independent products and one maximum, so that a warp that has a scheduler to itself waits
 // less): key_words(u, j, h, w) and value_words(u, m, w) give the f16 pairs w[0..7] of the lane's fragment of tile u
-// (kv8.cuh), `sk` the factor of the raw products, `lsv` log2 of the values' scale, `isv` its inverse, allowed(token)
-// the mask.
-template <int D, int N, bool MASK, typename KF, typename VF, typename AF>
-__device__ __forceinline__ void attend_tiles(Rows<D>& st, const uint32_t (&qf)[D / 64 * 4][4], const float (&sk)[N],
-                                             const float (&lsv)[N], const float (&isv)[N], int lane, KF key_words,
-                                             VF value_words, AF allowed) {
+// (kv8.cuh), `sk` the factor of the raw products, `lsv` log2 of the values' scale, `isv` its inverse, allowed(g, token)
+// the mask. qf[g][k step] is the fragment of the query rows.
+template <int D, int NG, int N, bool MASK, typename KF, typename VF, typename AF>
+__device__ __forceinline__ void attend_tiles(Rows<D, NG>& st, const uint32_t (&qf)[NG][D / 16][2],
+                                             const float (&sk)[NG][N], const float (&lsv)[N], const float (&isv)[N],
+                                             int lane, KF key_words, VF value_words, AF allowed) {
   constexpr int H = D / 64;
-  const int q = lane & 3;
-  float s[N][4][2];
-  float mx = -INFINITY;
+  const int r = lane >> 2;
+  float s[NG][N][4];
 #pragma unroll
   for (int u = 0; u < N; ++u)
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      float c[4] = {0.f, 0.f, 0.f, 0.f};
+    for (int jj = 0; jj < 2; ++jj) {
+      float c[NG][4];
+#pragma unroll
+      for (int g = 0; g < NG; ++g) c[g][0] = c[g][1] = c[g][2] = c[g][3] = 0.f;
 #pragma unroll
       for (int h = 0; h < H; ++h) {
-        uint32_t w[8];
-        key_words(u, j, h, w);
+        uint32_t w0[8], w1[8];
+        key_words(u, 2 * jj, h, w0);
+        key_words(u, 2 * jj + 1, h, w1);
 #pragma unroll
         for (int t = 0; t < 4; ++t)
-          mma16816(c, qf[h * 4 + t][0], qf[h * 4 + t][1], qf[h * 4 + t][2], qf[h * 4 + t][3], w[2 * t], w[2 * t + 1]);
+#pragma unroll
+          for (int g = 0; g < NG; ++g)
+            mma16816(c[g], w0[2 * t], w1[2 * t], w0[2 * t + 1], w1[2 * t + 1], qf[g][h * 4 + t][0], qf[g][h * 4 + t][1]);
       }
-      s[u][j][0] = fmaf(c[0] + c[2], sk[u], lsv[u]);
-      s[u][j][1] = fmaf(c[1] + c[3], sk[u], lsv[u]);
-      if (MASK) {
-        if (!allowed(8 * q + 2 * j)) s[u][j][0] = -INFINITY;
-        if (!allowed(8 * q + 2 * j + 1)) s[u][j][1] = -INFINITY;
+#pragma unroll
+      for (int g = 0; g < NG; ++g) {
+        s[g][u][2 * jj] = fmaf(c[g][0] + c[g][1], sk[g][u], lsv[u]);
+        s[g][u][2 * jj + 1] = fmaf(c[g][2] + c[g][3], sk[g][u], lsv[u]);
+        if (MASK) {
+          const int tok = 8 * (r >> 1) + 4 * jj + (r & 1);
+          if (!allowed(g, tok)) s[g][u][2 * jj] = -INFINITY;
+          if (!allowed(g, tok + 2)) s[g][u][2 * jj + 1] = -INFINITY;
+        }
       }
     }
+  float mn[NG];
+  bool grown = false;
 #pragma unroll
-  for (int u = 0; u < N; ++u)
+  for (int g = 0; g < NG; ++g) {
+    float mx = -INFINITY;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) mx = fmaxf(mx, fmaxf(s[u][j][0], s[u][j][1]));
-  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
-  mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-  const float mn = fmaxf(st.m, mx);
-  if (__any_sync(0xffffffffu, mn > st.m)) {
-    const float a = mn == -INFINITY ? 1.f : exp2_approx(st.m - mn);
-    st.l *= a;
+    for (int u = 0; u < N; ++u)
+      mx = fmaxf(mx, fmaxf(fmaxf(s[g][u][0], s[g][u][1]), fmaxf(s[g][u][2], s[g][u][3])));
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-#pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[n][i] *= a;
-    st.m = mn;
+    for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+    mn[g] = fmaxf(st.m[g], mx);
+    grown |= mn[g] > st.m[g];
   }
-  const float base = mn == -INFINITY ? 0.f : mn;  // a row that has seen no key yet: all weights 0
+  if (__any_sync(0xffffffffu, grown)) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      // O's columns are the rows' weights in two parts, in this lane those of row q: the factor is the lane's own
+      const float a = mn[g] == -INFINITY ? 1.f : exp2_approx(st.m[g] - mn[g]);
+      st.l[g] *= a;
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[g][n][i] *= a;
+      st.m[g] = mn[g];
+    }
+  }
 #pragma unroll
   for (int u = 0; u < N; ++u) {
-    uint32_t hi[4], lo[4];
-    float sum = 0.f;
+    uint32_t pf[NG][4];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const float w0 = exp2_approx(s[u][j][0] - base), w1 = exp2_approx(s[u][j][1] - base);
-      sum += w0 + w1;
-      split2(w0, w1, hi[j], lo[j]);
+    for (int g = 0; g < NG; ++g) {
+      const float base = mn[g] == -INFINITY ? 0.f : mn[g];  // a row that has seen no key yet: all weights 0
+      float sum = 0.f;
+#pragma unroll
+      for (int j = 0; j < 4; ++j) {
+        const float w = exp2_approx(s[g][u][j] - base);
+        sum += w;
+        pf[g][j] = transpose8(h2_u32(__floats2half2_rn(w, w - __half2float(__float2half_rn(w)))));
+      }
+      st.l[g] = fmaf(sum, isv[u], st.l[g]);
     }
-    st.l = fmaf(sum, isv[u], st.l);
 #pragma unroll
-    for (int m = 0; m < D / 16; ++m) {
+    for (int n = 0; n < D / 16; ++n) {
       uint32_t w[8];
-      value_words(u, m, w);
+      value_words(u, n, w);
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int i = 0; i < 2; ++i)
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
-          mma16816(st.o[2 * m + e], hi[2 * i], lo[2 * i], hi[2 * i + 1], lo[2 * i + 1], w[4 * e + 2 * i],
-                   w[4 * e + 2 * i + 1]);
+        for (int g = 0; g < NG; ++g)
+          mma16816(st.o[g][n], w[2 * i], w[4 + 2 * i], w[2 * i + 1], w[4 + 2 * i + 1], pf[g][2 * i], pf[g][2 * i + 1]);
     }
   }
 }
@@ -198,17 +230,18 @@ __device__ __forceinline__ int quotient(int a, int b) {
   return x + (rem >= b) - (rem < 0);
 }
 
-template <int D>
+template <int D, int NG>
 struct Smem {
-  static constexpr int CTAS_SM = D == 64 ? 3 : 2;
+  static constexpr int ROWS = 4 * NG;                                        // query rows of a unit
+  static constexpr int CTAS_SM = D == 64 ? (NG == 1 ? 4 : 3) : 2;
   static constexpr int SPLIT_COST = D == 64 ? 40 : 20;
-  static constexpr int STAGES = D == 64 ? 4 : 3;
-  static constexpr int PAIR = D == 64 ? 2 : 1;                // blocks of a step
-  static constexpr int HALF = BLOCK * D;      // a block's keys or values
-  static constexpr int STAGE = 2 * HALF;      // a block, or the keys or the values of a 16-bit tile
-  static constexpr int RING = STAGES * STAGE;  // of one warp
+  static constexpr int STAGES = D == 64 && NG == 2 ? 4 : 3;
+  static constexpr int PAIR = D == 64 && NG == 2 ? 2 : 1;                      // blocks of a step
+  static constexpr int HALF = BLOCK * D;                                     // a block's keys or values
+  static constexpr int STAGE = 2 * HALF;        // a block, or the keys or the values of a 16-bit tile
+  static constexpr int RING = STAGES * STAGE;   // of one warp
   static constexpr int PART = ROWS * D * 4 + ROWS * 8;  // a warp's rows of a unit: O, then (m, l)
-  static constexpr int HEAD = WARPS * RING;   // parts of units that go on from the piece before, one for each warp
+  static constexpr int HEAD = WARPS * RING;     // parts of units that go on from the piece before, one for each warp
   static constexpr int INFO = HEAD + WARPS * PART;
   static constexpr int TOTAL = INFO + WARPS * 2 * 32;
   static_assert(PART <= RING, "the other parts lie over the rings");
@@ -240,35 +273,39 @@ struct PartInfo {  // what a warp left in shared memory
   int valid, b, kvh, rb, first, last;
 };
 
-// Merged rows of a unit in the accumulators' layout: row r, columns 8n + 2q + {0, 1}.
-template <int D>
+// Merged rows of a unit: lane 4r + q has row 4g + q, columns 8n + r.
+template <int D, int NG>
 struct Merged {
-  float m, l;
-  float2 o[D / 8];
+  float m[NG], l[NG];
+  float o[NG][D / 8];
   __device__ __forceinline__ void clear() {
-    m = -INFINITY, l = 0.f;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) o[n] = make_float2(0.f, 0.f);
-  }
-  __device__ __forceinline__ void fold(float2 ml, const float2 (&v)[D / 8]) {
-    const float mn = fmaxf(m, ml.x);
-    const float base = mn == -INFINITY ? 0.f : mn;  // nothing but rows without a key so far
-    const float a = exp2_approx(m - base), e = exp2_approx(ml.x - base);
-    l = l * a + ml.y * e;
+    for (int g = 0; g < NG; ++g) {
+      m[g] = -INFINITY, l[g] = 0.f;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n) {
-      o[n].x = o[n].x * a + v[n].x * e;
-      o[n].y = o[n].y * a + v[n].y * e;
+      for (int n = 0; n < D / 8; ++n) o[g][n] = 0.f;
     }
-    m = mn;
+  }
+  __device__ __forceinline__ void fold(const float2 (&ml)[NG], const float (&v)[NG][D / 8]) {
+#pragma unroll
+    for (int g = 0; g < NG; ++g) {
+      const float mn = fmaxf(m[g], ml[g].x);
+      const float base = mn == -INFINITY ? 0.f : mn;  // nothing but rows without a key so far
+      const float a = exp2_approx(m[g] - base), e = exp2_approx(ml[g].x - base);
+      l[g] = l[g] * a + ml[g].y * e;
+#pragma unroll
+      for (int n = 0; n < D / 8; ++n) o[g][n] = o[g][n] * a + v[g][n] * e;
+      m[g] = mn;
+    }
   }
 };
 
 // RAGGED: every sequence has a position of its own.
-template <int DT, int FMT, int D, bool RAGGED>
-__global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kernel(const AttnParams p) {
+template <int DT, int FMT, int D, int NG, bool RAGGED>
+__global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_kernel(const AttnParams p) {
   extern __shared__ __align__(128) uint8_t smem[];
-  using S = Smem<D>;
+  using S = Smem<D, NG>;
+  constexpr int ROWS = S::ROWS;
   using T = typename Dt<DT>::T;
   constexpr int C16 = D / 8;
   constexpr int H = D / 64;
@@ -293,13 +330,16 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
     piece = quotient(total + ctas * WARPS - 1, ctas * WARPS);
     step = 1;
     if (n_units <= ctas) {
-      // A unit in CTAs of its own is merged without leaving the SM; equal pieces balance better, but end with a merge
-      // through L2 that takes as long as SPLIT_COST weights on an SM. 64 sequences of 4 kv heads at 511 (256 units):
-      // 15.1 us in equal pieces, 10.1 us with a CTA for each unit; at 8184 52.0 and 55 us.
-      const int own = max(PIECE_MIN, quotient(w + p.most_ctas * WARPS - 1, p.most_ctas * WARPS));
+      // A unit in CTAs of its own begins at once, and in one CTA is merged without leaving the SM; equal pieces balance
+      // better, but end with a merge through L2 that takes as long as SPLIT_COST weights on an SM. 64 sequences of 4
+      // kv heads (256 units) at 511: 15.1 us in equal pieces, 9.6 us with a CTA for each unit; at 8184 52 and 55 us.
+      // Several CTAs for a unit pay where they save a warp more than MERGE_COST weights.
+      int own = max(PIECE_MIN, quotient(w + p.most_ctas * WARPS - 1, p.most_ctas * WARPS));
+      const int alone = (w + WARPS - 1) / WARPS;
+      if (alone <= own + MERGE_COST) own = max(PIECE_MIN, alone);
       const int per_unit = quotient(w + own * WARPS - 1, own * WARPS);
-      const int sms = ctas / Smem<D>::CTAS_SM;
-      if (quotient(n_units * per_unit + sms - 1, sms) * (own * WARPS) <= quotient(total, sms) + Smem<D>::SPLIT_COST) {
+      const int sms = ctas / S::CTAS_SM;
+      if (quotient(n_units * per_unit + sms - 1, sms) * (own * WARPS) <= quotient(total, sms) + S::SPLIT_COST) {
         piece = own;
         step = own * WARPS;
         total = n_units * per_unit * step;
@@ -419,54 +459,66 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
   Segment g;
   bool more = next_segment(g);
   float2 sc = make_float2(0.f, 1.f);
-  uint4 q_raw[H][2];  // this lane's share of query row r
-  auto begin = [&]() {  // what a unit needs first, all in flight at once
+  uint4 q_raw[NG][H][2];  // this lane's share of query rows 4g + r / 2
+  auto begin = [&]() {    // what a unit needs first, all in flight at once
 #pragma unroll 1
     for (int j = 0; j < S::STAGES - 1; ++j) issue(g, j);
     sc = load_scale(g, g.lo);
-    const int gr = g.rb * ROWS + r, s = token_of(gr), head = g.kvh * p.groups + gr - s * p.groups;
-    const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(g.b) * p.seq + s) * p.qs +
-                   static_cast<int64_t>(head) * D;
 #pragma unroll
-    for (int h = 0; h < H; ++h)
+    for (int cg = 0; cg < NG; ++cg) {
+      const int gr = g.rb * ROWS + 4 * cg + (r >> 1), s = token_of(gr), head = g.kvh * p.groups + gr - s * p.groups;
+      const T* row = reinterpret_cast<const T*>(p.q) + (static_cast<int64_t>(g.b) * p.seq + s) * p.qs +
+                     static_cast<int64_t>(head) * D;
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
-        q_raw[h][e] = gr < p.rows ? __ldcg(reinterpret_cast<const uint4*>(row) + 8 * h + 2 * q + e)
-                                  : make_uint4(0, 0, 0, 0);
+      for (int h = 0; h < H; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          q_raw[cg][h][e] = gr < p.rows ? __ldcg(reinterpret_cast<const uint4*>(row) + 8 * h + 2 * q + e)
+                                        : make_uint4(0, 0, 0, 0);
+    }
   };
   if (more) begin();
   if (lane == 0) info[2 * warp].valid = info[2 * warp + 1].valid = 0;
 
-  auto store = [&](const Merged<D>& mg, int b_, int kvh_, int rb_) {
-    const int row = rb_ * ROWS + r;
-    if (row >= p.rows) return;
-    const float inv = 1.f / mg.l;
-    const int s = token_of(row), head = kvh_ * p.groups + row - s * p.groups;
-    T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b_) * p.seq + s) * p.os +
-             static_cast<int64_t>(head) * D + 2 * q;
+  auto store = [&](const Merged<D, NG>& mg, int b_, int kvh_, int rb_) {
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-      *reinterpret_cast<uint32_t*>(dst + 8 * n) = pack2<DT>(mg.o[n].x * inv, mg.o[n].y * inv);
+    for (int cg = 0; cg < NG; ++cg) {
+      const int row = rb_ * ROWS + 4 * cg + q;
+      const float inv = 1.f / mg.l[cg];
+      const int s = token_of(row), head = kvh_ * p.groups + row - s * p.groups;
+      T* dst = reinterpret_cast<T*>(p.out) + (static_cast<int64_t>(b_) * p.seq + s) * p.os +
+               static_cast<int64_t>(head) * D + (r & 1 ? 8 + r - 1 : r);
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {  // neighbouring columns lie in neighbouring r: a pair for each lane
+        const float v0 = mg.o[cg][2 * n] * inv, v1 = mg.o[cg][2 * n + 1] * inv;
+        const float other = __shfl_xor_sync(0xffffffffu, r & 1 ? v0 : v1, 4);
+        if (row < p.rows)
+          *reinterpret_cast<uint32_t*>(dst + 16 * n) = r & 1 ? pack2<DT>(other, v1) : pack2<DT>(v0, other);
+      }
+    }
   };
 
   while (more) {
     const int64_t bh = static_cast<int64_t>(g.b) * p.num_kv_heads + g.kvh;
-    // query rows: rotated, brought to the f16 range, split in two
-    const int gr = g.rb * ROWS + r;
-    const int qpos = gr < p.rows ? g.start + token_of(gr) : -1;  // a padding row sees no key of the 16-bit tiles, and
-    uint32_t qf[H * 4][4];                                        // its zeros harm nothing in the others
-    float cq;
-    {
-      float f[H][16];
+    // query rows: rotated, brought to the f16 range; even lanes r take f16(q), odd ones the remainder
+    uint32_t qf[NG][H * 4][2];
+    float cq[NG];
+    int qpos[NG];
+#pragma unroll
+    for (int cg = 0; cg < NG; ++cg) {
+      const int gr = g.rb * ROWS + 4 * cg + (r >> 1);
+      const int pos = gr < p.rows ? g.start + token_of(gr) : -1;  // a padding row sees no key of the 16-bit tiles, and
+      float f[H][16];                                             // its zeros harm nothing in the others
       float amax = 0.f;
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const uint32_t w[4] = {q_raw[h][e].x, q_raw[h][e].y, q_raw[h][e].z, q_raw[h][e].w};
+          const uint4 x = q_raw[cg][h][e];
+          const uint32_t w[4] = {x.x, x.y, x.z, x.w};
           float cc[4] = {1.f, 1.f, 1.f, 1.f}, ss[4] = {0.f, 0.f, 0.f, 0.f};
-          if (p.cos_t && qpos >= 0) {
-            const int64_t ang = static_cast<int64_t>(qpos) * (D / 2) + (8 * h + 2 * q + e) * 4;
+          if (p.cos_t && pos >= 0) {
+            const int64_t ang = static_cast<int64_t>(pos) * (D / 2) + (8 * h + 2 * q + e) * 4;
             const float4 a = __ldg(reinterpret_cast<const float4*>(p.cos_t + ang));
             const float4 d = __ldg(reinterpret_cast<const float4*>(p.sin_t + ang));
             cc[0] = a.x, cc[1] = a.y, cc[2] = a.z, cc[3] = a.w;
@@ -486,23 +538,31 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 1));
       amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, 2));
       const float up = to_f16_range(__float_as_uint(amax));
-      cq = p.scale_log2 / up;
+      // after the products lane 4r + q has row q, whose factor and position are in the lanes with r = 2q
+      cq[cg] = __shfl_sync(0xffffffffu, p.scale_log2 / up, 8 * q);
+      qpos[cg] = __shfl_sync(0xffffffffu, pos, 8 * q);
 #pragma unroll
       for (int h = 0; h < H; ++h)
 #pragma unroll
-        for (int t = 0; t < 4; ++t) {
-          split2(f[h][4 * t] * up, f[h][4 * t + 1] * up, qf[h * 4 + t][0], qf[h * 4 + t][1]);
-          split2(f[h][4 * t + 2] * up, f[h][4 * t + 3] * up, qf[h * 4 + t][2], qf[h * 4 + t][3]);
-        }
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {
+            uint32_t hi, lo;
+            split2(f[h][4 * t + 2 * e] * up, f[h][4 * t + 2 * e + 1] * up, hi, lo);
+            qf[cg][h * 4 + t][e] = r & 1 ? lo : hi;
+          }
     }
 
-    Rows<D> st;
-    st.m = -INFINITY;
-    st.l = 0.f;
+    Rows<D, NG> st;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
+    for (int cg = 0; cg < NG; ++cg) {
+      st.m[cg] = -INFINITY;
+      st.l[cg] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) st.o[n][i] = 0.f;
+      for (int n = 0; n < D / 16; ++n)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) st.o[cg][n][i] = 0.f;
+    }
 
     int j = 0;  // the slot that is read next; slots up to j + STAGES - 2 are on their way
     const int open = g.start % BLOCK, n8 = g.start / BLOCK;
@@ -550,8 +610,11 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
           return h2_u32(__floats2half2_rn(v.x * f, v.y * f));
         }
       };
-      const float sk1[1] = {cq / fk}, lsv1[1] = {-__log2f(fv)}, isv1[1] = {fv};
-      attend_tiles<D, 1, true>(
+      float sk1[NG][1];
+#pragma unroll
+      for (int cg = 0; cg < NG; ++cg) sk1[cg][0] = cq[cg] / fk;
+      const float lsv1[1] = {-__log2f(fv)}, isv1[1] = {fv};
+      attend_tiles<D, NG, 1, true>(
           st, qf, sk1, lsv1, isv1, lane,
           [&](int, int jj, int h, uint32_t (&w)[8]) {
             const int row = 8 * (r >> 1) + 2 * jj + (r & 1);
@@ -573,7 +636,7 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
               for (int i = 0; i < 4; ++i) w[4 * e + i] = to_half(x[i], fv);
             }
           },
-          [&](int token) { return (n8 + t) * BLOCK + token <= qpos; });
+          [&](int cg, int token) { return (n8 + t) * BLOCK + token <= qpos[cg]; });
 
       if (p.seq == 1 && g.rb == 0) {  // the append of a decode step
         T* to_row = reinterpret_cast<T*>(p.tail) + bh * 2 * BLOCK * D;
@@ -611,17 +674,19 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
       issue(g, j + S::STAGES - 1);
       cp_async_wait<S::STAGES - N>();
       __syncwarp();  // every lane's copies of the blocks have landed
-      float sk[N], lsv[N], isv[N];
+      float sk[NG][N], lsv[N], isv[N];
 #pragma unroll
       for (int u = 0; u < N; ++u) {
-        sk[u] = cq * __shfl_sync(0xffffffffu, sc.x, i + u);
+        const float x = __shfl_sync(0xffffffffu, sc.x, i + u);
+#pragma unroll
+        for (int cg = 0; cg < NG; ++cg) sk[cg][u] = cq[cg] * x;
         lsv[u] = __shfl_sync(0xffffffffu, lv_l, i + u);
         isv[u] = __shfl_sync(0xffffffffu, iv_l, i + u);
       }
       const uint8_t* slot[N];
 #pragma unroll
       for (int u = 0; u < N; ++u) slot[u] = ring + ((j + u) % S::STAGES) * S::STAGE + lane * 16;
-      attend_tiles<D, N, false>(
+      attend_tiles<D, NG, N, false>(
           st, qf, sk, lsv, isv, lane,
           [&](int u, int jj, int h, uint32_t (&w)[8]) {
             const uint4 x = *reinterpret_cast<const uint4*>(slot[u] + (jj * H + h) * 512);
@@ -637,7 +702,7 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
             decode4<FMT>(x.z, w[4], w[5]);
             decode4<FMT>(x.w, w[6], w[7]);
           },
-          [](int) { return true; });
+          [](int, int) { return true; });
       __syncwarp();  // the slots are written again by the next copies
       if constexpr (N == 2) issue(g, j + S::STAGES);
       j += N;
@@ -655,13 +720,19 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
     more = next_segment(g);
     if (more) begin();
 
-    Merged<D> mg;
-    mg.m = st.m;
-    mg.l = st.l + __shfl_xor_sync(0xffffffffu, st.l, 1);
-    mg.l += __shfl_xor_sync(0xffffffffu, mg.l, 2);
+    Merged<D, NG> mg;
 #pragma unroll
-    for (int n = 0; n < D / 8; ++n)
-      mg.o[n] = make_float2(st.o[n][0] + st.o[n][2], st.o[n][1] + st.o[n][3]);
+    for (int cg = 0; cg < NG; ++cg) {
+      mg.m[cg] = st.m[cg];
+      mg.l[cg] = st.l[cg];
+#pragma unroll
+      for (int o = 4; o < 32; o <<= 1) mg.l[cg] += __shfl_xor_sync(0xffffffffu, mg.l[cg], o);
+#pragma unroll
+      for (int n = 0; n < D / 16; ++n) {
+        mg.o[cg][2 * n] = st.o[cg][n][0] + st.o[cg][n][1];
+        mg.o[cg][2 * n + 1] = st.o[cg][n][2] + st.o[cg][n][3];
+      }
+    }
     if (done.first == done.last) {
       store(mg, done.b, done.kvh, done.rb);
     } else {
@@ -669,8 +740,13 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
       const int k = me == done.first;
       uint8_t* part = k ? ring : smem + S::HEAD + warp * S::PART;
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) *reinterpret_cast<float2*>(part + (n * 32 + lane) * 8) = mg.o[n];
-      if (q == 0) *reinterpret_cast<float2*>(part + ROWS * D * 4 + r * 8) = make_float2(mg.m, mg.l);
+      for (int cg = 0; cg < NG; ++cg) {
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          *reinterpret_cast<float*>(part + ((cg * (D / 8) + n) * 32 + lane) * 4) = mg.o[cg][n];
+        if (r == 0)
+          *reinterpret_cast<float2*>(part + ROWS * D * 4 + (4 * cg + q) * 8) = make_float2(mg.m[cg], mg.l[cg]);
+      }
       if (lane == 0) info[2 * warp + k] = PartInfo{1, done.b, done.kvh, done.rb, done.first, done.last};
     }
   }
@@ -689,25 +765,34 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
     const int w0 = k ? warp : 0;  // where the unit's parts begin
     const PartInfo u = info[2 * w0 + k];
     if (!u.valid || (k == 0 && warp != head_by)) continue;
-    Merged<D> mg;
+    Merged<D, NG> mg;
     mg.clear();
     for (int w = w0; w < WARPS; ++w) {
       const int kk = w == w0 ? k : 0;
       if (w > w0 && blockIdx.x * WARPS + w > u.last) break;
       const uint8_t* part = kk ? smem + w * S::RING : smem + S::HEAD + w * S::PART;
-      float2 v[D / 8];
+      float2 ml[NG];
+      float v[NG][D / 8];
 #pragma unroll
-      for (int n = 0; n < D / 8; ++n) v[n] = *reinterpret_cast<const float2*>(part + (n * 32 + lane) * 8);
-      mg.fold(*reinterpret_cast<const float2*>(part + ROWS * D * 4 + r * 8), v);
+      for (int cg = 0; cg < NG; ++cg) {
+        ml[cg] = *reinterpret_cast<const float2*>(part + ROWS * D * 4 + (4 * cg + q) * 8);
+#pragma unroll
+        for (int n = 0; n < D / 8; ++n)
+          v[cg][n] = *reinterpret_cast<const float*>(part + ((cg * (D / 8) + n) * 32 + lane) * 4);
+      }
+      mg.fold(ml, v);
     }
     const int c_first = u.first / WARPS, c_last = u.last / WARPS;
     if (c_first != c_last) {
       auto slot_of = [&](int c) { return 2 * static_cast<int64_t>(c) + (c == c_first); };
       auto put = [&](int c) {
         const int64_t slot = slot_of(c);
-        if (q == 0) p.part_ml[slot * ROWS + r] = make_float2(mg.m, mg.l);
 #pragma unroll
-        for (int n = 0; n < D / 8; ++n) p.part_o[(slot * (D / 8) + n) * 32 + lane] = mg.o[n];
+        for (int cg = 0; cg < NG; ++cg) {
+          if (r == 0) p.part_ml[(slot * NG + cg) * 4 + q] = make_float2(mg.m[cg], mg.l[cg]);
+#pragma unroll
+          for (int n = 0; n < D / 8; ++n) p.part_o[((slot * NG + cg) * (D / 8) + n) * 32 + lane] = mg.o[cg][n];
+        }
       };
       auto arrive = [&](int* counter, int count) {  // whether this warp is the last of `count`
         int last = 0;
@@ -725,17 +810,22 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
         return last != 0;
       };
       auto gather = [&](int count, auto cta_of) {  // parts of CTAs cta_of(0 .. count - 1), in this order
-        constexpr int AHEAD = D == 64 ? 4 : 2;
+        constexpr int AHEAD = 256 / (D * NG);
         mg.clear();
 #pragma unroll 1
         for (int i0 = 0; i0 < count; i0 += AHEAD) {
-          float2 ml[AHEAD], v[AHEAD][D / 8];
+          float2 ml[AHEAD][NG];
+          float v[AHEAD][NG][D / 8];
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i) {
             const int64_t slot = slot_of(cta_of(min(i0 + i, count - 1)));
-            ml[i] = __ldcg(p.part_ml + slot * ROWS + r);
 #pragma unroll
-            for (int n = 0; n < D / 8; ++n) v[i][n] = __ldcg(p.part_o + (slot * (D / 8) + n) * 32 + lane);
+            for (int cg = 0; cg < NG; ++cg) {
+              ml[i][cg] = __ldcg(p.part_ml + (slot * NG + cg) * 4 + q);
+#pragma unroll
+              for (int n = 0; n < D / 8; ++n)
+                v[i][cg][n] = __ldcg(p.part_o + ((slot * NG + cg) * (D / 8) + n) * 32 + lane);
+            }
           }
 #pragma unroll
           for (int i = 0; i < AHEAD; ++i)
@@ -762,35 +852,54 @@ __global__ void __launch_bounds__(THREADS, Smem<D>::CTAS_SM) kv8_attention_kerne
 
 // The arrival counters come first, then two slots of rows for each CTA: one size for all shapes of a head_dim, so
 // calls that follow one another on a stream can share one workspace.
-int total_ctas(int head_dim, int sm_count) {
-  return (head_dim == 64 ? Smem<64>::CTAS_SM : Smem<128>::CTAS_SM) * std::max(sm_count, 1);
+int64_t counter_bytes(int sm_count) { return (int64_t(4) * sm_count * 3 * sizeof(int) + 255) / 256 * 256; }
+template <int D, int NG>
+int64_t parts_bytes(int sm_count) {
+  return int64_t(Smem<D, NG>::CTAS_SM) * sm_count * 2 * Smem<D, NG>::PART;
 }
-int64_t counter_bytes(int ctas) { return (int64_t(ctas) * 3 * sizeof(int) + 255) / 256 * 256; }
 int64_t workspace_bytes_for(int head_dim, int sm_count) {
-  const int ctas = total_ctas(head_dim, sm_count);
-  return counter_bytes(ctas) + int64_t(ctas) * 2 * ROWS * (sizeof(float2) + sizeof(float) * head_dim);
+  return counter_bytes(sm_count) + (head_dim == 64 ? std::max(parts_bytes<64, 1>(sm_count), parts_bytes<64, 2>(sm_count))
+                                                   : std::max(parts_bytes<128, 1>(sm_count), parts_bytes<128, 2>(sm_count)));
 }
 
-template <int DT, int FMT, int D, bool RAGGED>
-int launch(const AttnParams& p, int ctas, cudaStream_t st) {
-  auto kern = kv8_attention_kernel<DT, FMT, D, RAGGED>;
+template <int DT, int FMT, int D, int NG, bool RAGGED>
+int launch(AttnParams& p, void* workspace, const DeviceInfo& dev, cudaStream_t st) {
+  using S = Smem<D, NG>;
+  auto kern = kv8_attention_kernel<DT, FMT, D, NG, RAGGED>;
   static bool configured[64] = {};
-  DeviceInfo dev;
-  if (int rc = current_device_info(&dev)) return rc;
   if (!configured[dev.device]) {
-    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, Smem<D>::TOTAL),
+    if (int rc = check_cuda(cudaFuncSetAttribute(kern, cudaFuncAttributeMaxDynamicSharedMemorySize, S::TOTAL),
                             "cudaFuncSetAttribute(kv8_attention)"))
       return rc;
     configured[dev.device] = true;
   }
-  return launch_kernel(kern, dim3(ctas), dim3(THREADS), Smem<D>::TOTAL, st, 1, "kv8_attention", p);
+  const int ctas = S::CTAS_SM * std::max(dev.sm_count, 1);
+  p.n_rb = (p.rows + S::ROWS - 1) / S::ROWS;
+  // the line of tiles is counted in 32 bits
+  const int64_t units = int64_t(p.batch) * p.num_kv_heads * p.n_rb;
+  const int64_t longest = UNIT_WEIGHT + p.num_blocks + int64_t(TAIL_WEIGHT) * (p.seq / BLOCK + 2) + WARPS * PIECE_MIN;
+  if (units > INT32_MAX / longest) return fail_invalid("kv8_attention: too many query rows for one call");
+  p.most_ctas = static_cast<int>(std::max<int64_t>(1, ctas / units));
+  char* ws = static_cast<char*>(workspace);
+  p.counters = reinterpret_cast<int*>(ws);
+  ws += counter_bytes(dev.sm_count);
+  p.part_ml = reinterpret_cast<float2*>(ws);
+  ws += int64_t(ctas) * 2 * S::ROWS * sizeof(float2);
+  p.part_o = reinterpret_cast<float*>(ws);
+  return launch_kernel(kern, dim3(ctas), dim3(THREADS), S::TOTAL, st, 1, "kv8_attention", p);
+}
+
+template <int DT, int FMT, int D>
+int launch(AttnParams& p, void* workspace, const DeviceInfo& dev, cudaStream_t st) {
+  const bool ragged = p.start_dev && p.start_step;
+  if (p.rows <= 4)
+    return ragged ? launch<DT, FMT, D, 1, true>(p, workspace, dev, st) : launch<DT, FMT, D, 1, false>(p, workspace, dev, st);
+  return ragged ? launch<DT, FMT, D, 2, true>(p, workspace, dev, st) : launch<DT, FMT, D, 2, false>(p, workspace, dev, st);
 }
 
 template <int DT, int FMT>
-int launch(const AttnParams& p, int head_dim, int ctas, cudaStream_t st) {
-  const bool ragged = p.start_dev && p.start_step;
-  if (head_dim == 64) return ragged ? launch<DT, FMT, 64, true>(p, ctas, st) : launch<DT, FMT, 64, false>(p, ctas, st);
-  return ragged ? launch<DT, FMT, 128, true>(p, ctas, st) : launch<DT, FMT, 128, false>(p, ctas, st);
+int launch(AttnParams& p, int head_dim, void* workspace, const DeviceInfo& dev, cudaStream_t st) {
+  return head_dim == 64 ? launch<DT, FMT, 64>(p, workspace, dev, st) : launch<DT, FMT, 128>(p, workspace, dev, st);
 }
 
 }  // namespace kv8
@@ -841,14 +950,10 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   DeviceInfo di;
   if (int rc = current_device_info(&di)) return rc;
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
-  // the line of tiles is counted in 32 bits
-  const int64_t units = int64_t(batch) * num_kv_heads * ((rows + ROWS - 1) / ROWS);
-  const int64_t longest = UNIT_WEIGHT + num_blocks + int64_t(TAIL_WEIGHT) * (seq / BLOCK + 2) + WARPS * PIECE_MIN;
-  if (units > INT32_MAX / longest) return fail_invalid("kv8_attention: too many query rows for one call");
+  if (rows > INT32_MAX) return fail_invalid("kv8_attention: too many query rows for one call");
   if (!workspace || workspace_bytes < workspace_bytes_for(head_dim, di.sm_count))
     return fail_invalid("kv8_attention: workspace missing or smaller than tk_kv8_attention_workspace()");
   if (!aligned16(workspace)) return fail_invalid("kv8_attention: workspace must be 16-byte aligned");
-  const int ctas = total_ctas(head_dim, di.sm_count);
   AttnParams p{};
   p.q = q;
   p.qs = q_tok_stride;
@@ -873,24 +978,16 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   p.start_pos = start_pos;
   p.start_dev = start_pos_device;
   p.start_step = start_pos_step;
-  p.n_rb = static_cast<int>((rows + ROWS - 1) / ROWS);
   p.batch = batch;
-  p.most_ctas = static_cast<int>(std::max<int64_t>(1, ctas / units));
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
-  char* ws = static_cast<char*>(workspace);
-  p.counters = reinterpret_cast<int*>(ws);
-  ws += counter_bytes(ctas);
-  p.part_ml = reinterpret_cast<float2*>(ws);
-  ws += int64_t(ctas) * 2 * ROWS * sizeof(float2);
-  p.part_o = reinterpret_cast<float2*>(ws);
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (dtype == TK_F16)
-    rc = format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, head_dim, ctas, st)
-                               : launch<TK_F16, TK_KV8_INT8>(p, head_dim, ctas, st);
+    rc = format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, head_dim, workspace, di, st)
+                               : launch<TK_F16, TK_KV8_INT8>(p, head_dim, workspace, di, st);
   else
-    rc = format == TK_KV8_E4M3 ? launch<TK_BF16, TK_KV8_E4M3>(p, head_dim, ctas, st)
-                               : launch<TK_BF16, TK_KV8_INT8>(p, head_dim, ctas, st);
+    rc = format == TK_KV8_E4M3 ? launch<TK_BF16, TK_KV8_E4M3>(p, head_dim, workspace, di, st)
+                               : launch<TK_BF16, TK_KV8_INT8>(p, head_dim, workspace, di, st);
   if (rc || seq == 1) return rc;
   return append(c, k, k_tok_stride, v, v_tok_stride, cos_table, sin_table, table_rows, batch, seq, num_kv_heads,
                 head_dim, start_pos, start_pos_device, start_pos_step, dtype, st);
