@@ -18,6 +18,19 @@ def call_ctx(dev: torch.device):
     return torch.cuda.device(idx)
 
 
+def launch(idx: int, what: str, kernels: int, fn, *args) -> None:
+    """Call a library entry point on device ``idx`` and its current stream (the call's last argument);
+    raises on an error status, counts the kernels otherwise."""
+    if torch._C._cuda_getDevice() == idx:
+        rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    else:
+        with torch.cuda.device(idx):
+            rc = fn(*args, torch._C._cuda_getCurrentRawStream(idx))
+    if rc:
+        _lib.check(rc, what)
+    _lib.launch_counter[0] += kernels
+
+
 def rows_view(x: torch.Tensor) -> torch.Tensor:
     """2-D [rows, last] view whose last dim is contiguous (copies only if it must)."""
     x2 = x.reshape(-1, x.shape[-1])
@@ -56,4 +69,4 @@ def weights_are_stable() -> bool:
     return getattr(_graph_state, "stable", False)
 
 
-__all__ = ["call_ctx", "rows_view", "row_stride", "ptr", "_lib", "stable_weights", "weights_are_stable"]
+__all__ = ["call_ctx", "launch", "rows_view", "row_stride", "ptr", "_lib", "stable_weights", "weights_are_stable"]

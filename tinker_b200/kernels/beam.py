@@ -8,10 +8,21 @@ The reference has neither a KV cache nor a decoding loop (eb1386/TinKer README.m
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from tinker_b200 import _lib
-from tinker_b200.kernels._common import call_ctx
+from tinker_b200.kernels._common import launch
+
+
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(idx: int, batch: int, beams: int, vocab: int, num_select: int) -> int:
+    with torch.cuda.device(idx):
+        n = _lib.lib().tk_beam_select_workspace(batch, beams, vocab, num_select)
+    if n < 0:
+        raise RuntimeError(f"tk_beam_select_workspace: {_lib.last_error()}")
+    return n
 
 
 def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_select: int | None = None,
@@ -26,7 +37,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_select: int | No
     all its tokens are worth -inf, like NaN and -inf logits; a +inf logit counts as the largest finite
     value. Returns ``(scores float32, beams int64, tokens int64)``, each [batch, num_select].
     """
-    dev = _lib.require_cuda(logits, scores)
+    idx = _lib.cuda_index(logits, scores)
     if logits.dim() != 3:
         raise ValueError(f"beam_select: logits must be [batch, beams, vocab], got {tuple(logits.shape)}")
     B, K, V = logits.shape
@@ -37,7 +48,7 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_select: int | No
         raise ValueError(f"beam_select: cannot select {n} of {K} x {V} continuations")
     fin_ptr, eos = None, -1
     if finished is not None:
-        _lib.require_cuda(logits, finished)
+        _lib.cuda_index(logits, finished)
         if finished.shape != (B, K) or finished.dtype is not torch.bool:
             raise ValueError(f"beam_select: finished must be bool [{B}, {K}]")
         if eos_token_id is None or not 0 <= int(eos_token_id) < V:
@@ -50,19 +61,16 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_select: int | No
         logits = logits.contiguous()
         row = V
     scores = scores.contiguous()
-    out = torch.empty((B, n), dtype=torch.float32, device=logits.device)
-    beams = torch.empty((B, n), dtype=torch.int64, device=logits.device)
-    tokens = torch.empty((B, n), dtype=torch.int64, device=logits.device)
+    out = scores.new_empty((B, n))
+    beams = torch.empty((B, n), dtype=torch.int64, device=out.device)
+    tokens = torch.empty_like(beams)
     if B == 0:
         return out, beams, tokens
-    lib = _lib.lib()
-    with call_ctx(dev):
-        need = lib.tk_beam_select_workspace(B, K, V, n)
-        ws = torch.empty(max(need, 0), dtype=torch.uint8, device=logits.device)
-        _lib.check(lib.tk_beam_select(
-            logits.data_ptr(), row, scores.data_ptr(), fin_ptr, eos, out.data_ptr(), beams.data_ptr(),
-            tokens.data_ptr(), B, K, V, n, ws.data_ptr(), need, _lib.dtype_code(logits.dtype),
-            _lib.stream_ptr(dev)), "tk_beam_select", 2)
+    need = _workspace_bytes(idx, B, K, V, n)
+    ws = torch.empty(need, dtype=torch.uint8, device=out.device)
+    launch(idx, "tk_beam_select", 2, _lib.lib().tk_beam_select, logits.data_ptr(), row, scores.data_ptr(), fin_ptr, eos,
+           out.data_ptr(), beams.data_ptr(), tokens.data_ptr(), B, K, V, n, ws.data_ptr(), need,
+           _lib.dtype_code(logits.dtype))
     return out, beams, tokens
 
 
@@ -93,7 +101,7 @@ def kv_reorder(k_cache: torch.Tensor, v_cache: torch.Tensor, parents: torch.Tens
     dimension; parents: int64 [groups, beams], groups * beams = rows, at most 32 beams. A group with a
     parent outside its beams stays as it is and device error 4 is recorded.
     """
-    dev = _lib.require_cuda(k_cache, v_cache, parents)
+    idx = _lib.cuda_index(k_cache, v_cache, parents)
     if k_cache.dim() not in (4, 5) or k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
         raise ValueError("kv_reorder: k_cache and v_cache must both be [(layers,) rows, heads, capacity, head_dim]")
     if k_cache.dtype not in (torch.float16, torch.bfloat16):
@@ -107,18 +115,16 @@ def kv_reorder(k_cache: torch.Tensor, v_cache: torch.Tensor, parents: torch.Tens
     groups, beams = parents.shape
     if rows == 0 or layers == 0 or heads == 0 or d == 0:
         return
-    with call_ctx(dev):
-        _lib.check(_lib.lib().tk_kv_reorder(
-            k_cache.data_ptr(), v_cache.data_ptr(), parents.data_ptr(), layers, groups, beams, heads, cap, d, n,
-            n_ptr, _lib.dtype_code(k_cache.dtype), _lib.stream_ptr(dev)), "tk_kv_reorder",
-            1 if beams > 1 and (n or n_ptr) else 0)
+    launch(idx, "tk_kv_reorder", 1 if beams > 1 and (n or n_ptr) else 0, _lib.lib().tk_kv_reorder, k_cache.data_ptr(),
+           v_cache.data_ptr(), parents.data_ptr(), layers, groups, beams, heads, cap, d, n, n_ptr,
+           _lib.dtype_code(k_cache.dtype))
 
 
 def kv8_reorder(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tensor, tail: torch.Tensor,
                 parents: torch.Tensor, length) -> None:
     """``kv_reorder`` of an 8-bit cache (``kernels/kv_cache8.py``): the blocks, scales and open rows
     that hold positions below ``length``. The tensors may have a leading layer dimension."""
-    dev = _lib.require_cuda(k_cache, v_cache, scales, tail, parents)
+    idx = _lib.cuda_index(k_cache, v_cache, scales, tail, parents)
     lead = k_cache.shape[:-3]
     if k_cache.dim() not in (4, 5) or k_cache.shape != v_cache.shape or k_cache.dtype is not v_cache.dtype:
         raise ValueError("kv8_reorder: k_cache and v_cache must both be [(layers,) rows, heads, blocks, 32 * head_dim]")
@@ -138,8 +144,6 @@ def kv8_reorder(k_cache: torch.Tensor, v_cache: torch.Tensor, scales: torch.Tens
     groups, beams = parents.shape
     if rows == 0 or layers == 0 or heads == 0 or d == 0:
         return
-    with call_ctx(dev):
-        _lib.check(_lib.lib().tk_kv8_reorder(
-            k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), tail.data_ptr(), parents.data_ptr(), layers,
-            groups, beams, heads, nb, d, n, n_ptr, _lib.stream_ptr(dev)), "tk_kv8_reorder",
-            1 if beams > 1 and (n or n_ptr) else 0)
+    launch(idx, "tk_kv8_reorder", 1 if beams > 1 and (n or n_ptr) else 0, _lib.lib().tk_kv8_reorder, k_cache.data_ptr(),
+           v_cache.data_ptr(), scales.data_ptr(), tail.data_ptr(), parents.data_ptr(), layers, groups, beams, heads, nb,
+           d, n, n_ptr)

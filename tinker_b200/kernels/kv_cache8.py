@@ -21,11 +21,12 @@ left in the tail. A cache may start over at 0 or at any multiple of 32 that it h
 
 from __future__ import annotations
 
+import functools
+
 import torch
 
 from tinker_b200 import _lib
-from tinker_b200.kernels._common import call_ctx
-from tinker_b200.kernels.fused_attention import _token_stride
+from tinker_b200.kernels._common import launch
 
 KV8_BLOCK = 32
 KV8_FORMATS = {torch.float8_e4m3fn: 0, torch.int8: 1}
@@ -62,12 +63,23 @@ def kv8_attention_workspace(batch: int, num_heads: int, num_kv_heads: int, head_
     return int(n)
 
 
+@functools.lru_cache(maxsize=64)
+def _workspace_bytes(idx: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """``kv8_attention_workspace`` on device ``idx``; the size does not depend on the other arguments."""
+    with torch.cuda.device(idx):
+        return kv8_attention_workspace(1, num_heads, num_kv_heads, head_dim, 1, 1)
+
+
 def _rows(t: torch.Tensor, B: int, S: int, width: int) -> tuple[torch.Tensor, int]:
-    """``_token_stride`` whose copy is also made where the rows do not start on 16 bytes."""
-    t, stride = _token_stride(t, B, S, width)
-    if t.data_ptr() % 16:
-        t, stride = t.clone(memory_format=torch.contiguous_format), width
-    return t, stride
+    """(tensor, token stride) of [B, S, width] rows that start on 16 bytes and follow one another at one
+    stride; anything else is copied."""
+    if t.shape != (B, S, width):
+        raise ValueError(f"expected shape ({B}, {S}, {width}), got {tuple(t.shape)}")
+    s0, s1, s2 = t.stride()
+    tok = s1 if S > 1 else (s0 if B > 1 else width)
+    if s2 == 1 and tok >= width and tok % 8 == 0 and (B == 1 or S == 1 or s0 == S * s1) and t.data_ptr() % 16 == 0:
+        return t, tok
+    return t.clone(memory_format=torch.contiguous_format), width
 
 
 def _check_cache(what: str, k_cache, v_cache, scales, tail, batch: int, heads: int, head_dim: int,
@@ -108,82 +120,75 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
     later calls of any shape can use it, but not calls that overlap in time (allocated per call when
     omitted). Returns [B, S, num_heads * head_dim] in q's dtype.
     """
-    dev = _lib.require_cuda(q, k, v, k_cache, v_cache, scales, tail)
-    B, S = q.shape[0], q.shape[1]
-    if k.dtype is not q.dtype or v.dtype is not q.dtype:
-        raise TypeError("kv8_attention: q, k, v must all be float16 or all bfloat16")
-    nb, code = _check_cache("kv8_attention", k_cache, v_cache, scales, tail, B, num_kv_heads, head_dim, q.dtype)
-    q3, qs = _rows(q, B, S, num_heads * head_dim)
-    k3, ks = _rows(k, B, S, num_kv_heads * head_dim)
-    v3, vs = _rows(v, B, S, num_kv_heads * head_dim)
+    idx = _lib.cuda_index(q, k, v, k_cache, v_cache, scales, tail)
+    dtype = q.dtype
+    if q.dim() != 3 or k.dtype is not dtype or v.dtype is not dtype:
+        raise TypeError("kv8_attention: q, k, v must be [batch, seq, heads * head_dim], all float16 or all bfloat16")
+    B, S, width = q.shape
+    nb, code = _check_cache("kv8_attention", k_cache, v_cache, scales, tail, B, num_kv_heads, head_dim, dtype)
+    q, qs = _rows(q, B, S, num_heads * head_dim)
+    k, ks = _rows(k, B, S, num_kv_heads * head_dim)
+    v, vs = _rows(v, B, S, num_kv_heads * head_dim)
     cos_ptr = sin_ptr = None
     rows = 0
     if cos_table is not None or sin_table is not None:
         if cos_table is None or sin_table is None:
             raise ValueError("kv8_attention: give both RoPE tables or neither")
-        _lib.require_cuda(q, cos_table, sin_table)
+        _lib.cuda_index(q, cos_table, sin_table)
         if cos_table.dtype is not torch.float32 or sin_table.dtype is not torch.float32:
             raise TypeError("kv8_attention: the RoPE tables must be float32")
-        c, s = cos_table.contiguous(), sin_table.contiguous()
-        if c.shape != s.shape or c.dim() != 2 or c.shape[1] != head_dim // 2:
-            raise ValueError(f"RoPE tables must be [max_seq_len, {head_dim // 2}], got {tuple(c.shape)}")
-        cos_ptr, sin_ptr, rows = c.data_ptr(), s.data_ptr(), c.shape[0]
+        if cos_table.dim() != 2 or cos_table.shape[1] != head_dim // 2 or sin_table.shape != cos_table.shape:
+            raise ValueError(f"RoPE tables must be [max_seq_len, {head_dim // 2}], got {tuple(cos_table.shape)}")
+        cos_table, sin_table = cos_table.contiguous(), sin_table.contiguous()
+        cos_ptr, sin_ptr, rows = cos_table.data_ptr(), sin_table.data_ptr(), cos_table.shape[0]
     pos_ptr, step = None, 0
     if position is not None:
         n = position.numel()
-        if position.dtype is not torch.int32 or position.device != q.device or n not in (1, B):
+        if position.dtype is not torch.int32 or position.get_device() != idx or n not in (1, B):
             raise TypeError("kv8_attention: position must be an int32 tensor on q's device with 1 or batch elements")
         if n > 1:
             position = position.contiguous()
             step = 1
-        pos_ptr, start_pos, max_kv = position.data_ptr(), 0, nb * KV8_BLOCK
+        pos_ptr, start_pos = position.data_ptr(), 0
     else:
         start_pos = int(start_pos)
-        max_kv = start_pos + S
-        if start_pos < 0 or max_kv > nb * KV8_BLOCK:
-            raise ValueError(f"kv8_attention: positions {start_pos}..{max_kv - 1} exceed the cache capacity "
+        if start_pos < 0 or start_pos + S > nb * KV8_BLOCK:
+            raise ValueError(f"kv8_attention: positions {start_pos}..{start_pos + S - 1} exceed the cache capacity "
                              f"{nb * KV8_BLOCK}")
-    out = torch.empty((B, S, num_heads * head_dim), dtype=q.dtype, device=q.device)
+    out = q.new_empty((B, S, width))
     if B == 0 or S == 0:
         return out
-    lib = _lib.lib()
-    with call_ctx(dev):
-        need = kv8_attention_workspace(B, num_heads, num_kv_heads, head_dim, S, max_kv)
-        ws_ptr = None
-        if need > 0:
-            if workspace is None:
-                workspace = torch.zeros(need, dtype=torch.uint8, device=q.device)
-            elif workspace.numel() * workspace.element_size() < need or workspace.device != q.device:
-                raise ValueError(f"kv8_attention: workspace smaller than the {need} bytes needed")
-            ws_ptr = workspace.data_ptr()
-        _lib.check(lib.tk_kv8_attention(
-            q3.data_ptr(), qs, k3.data_ptr(), ks, v3.data_ptr(), vs, k_cache.data_ptr(), v_cache.data_ptr(),
-            scales.data_ptr(), tail.data_ptr(), nb, code, cos_ptr, sin_ptr, rows, out.data_ptr(),
-            num_heads * head_dim, B, S, num_heads, num_kv_heads, head_dim, start_pos, pos_ptr, step, ws_ptr, need,
-            _lib.dtype_code(q.dtype), _lib.stream_ptr(dev)), "tk_kv8_attention", 1 if S == 1 else 2)
+    need = _workspace_bytes(idx, num_heads, num_kv_heads, head_dim)
+    if workspace is None:
+        workspace = torch.zeros(need, dtype=torch.uint8, device=out.device)
+    elif workspace.nbytes < need or workspace.get_device() != idx or not workspace.is_contiguous():
+        raise ValueError(f"kv8_attention: workspace smaller than the {need} bytes needed, or not contiguous")
+    launch(idx, "tk_kv8_attention", 1 if S == 1 else 2, _lib.lib().tk_kv8_attention, q.data_ptr(), qs, k.data_ptr(), ks,
+           v.data_ptr(), vs, k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), tail.data_ptr(), nb, code,
+           cos_ptr, sin_ptr, rows, out.data_ptr(), width, B, S, num_heads, num_kv_heads, head_dim, start_pos, pos_ptr,
+           step, workspace.data_ptr(), need, _lib.dtype_code(dtype))
     return out
 
 
 def kv8_append(k, v, k_cache, v_cache, scales, tail, start_pos: int = 0) -> None:
     """Append k (already rotated) and v, [B, S, num_kv_heads * head_dim], at ``start_pos``."""
-    dev = _lib.require_cuda(k, v, k_cache, v_cache, scales, tail)
+    idx = _lib.cuda_index(k, v, k_cache, v_cache, scales, tail)
     if k.dim() != 3 or k_cache.dim() != 4 or v.dtype is not k.dtype:
         raise ValueError("kv8_append: k and v must be [batch, seq, heads * head_dim] of one type, the cache "
                          "[batch, heads, blocks, 32 * head_dim]")
-    B, S = k.shape[0], k.shape[1]
-    hkv, D = k_cache.shape[1], k_cache.shape[3] // KV8_BLOCK
+    B, S, _ = k.shape
+    _, hkv, _, block = k_cache.shape
+    D = block // KV8_BLOCK
     nb, code = _check_cache("kv8_append", k_cache, v_cache, scales, tail, B, hkv, D, k.dtype)
-    k3, ks = _rows(k, B, S, hkv * D)
-    v3, vs = _rows(v, B, S, hkv * D)
+    k, ks = _rows(k, B, S, hkv * D)
+    v, vs = _rows(v, B, S, hkv * D)
     start_pos = int(start_pos)
     if start_pos < 0 or start_pos + S > nb * KV8_BLOCK:
         raise ValueError(f"kv8_append: positions {start_pos}..{start_pos + S - 1} exceed the cache capacity "
                          f"{nb * KV8_BLOCK}")
-    with call_ctx(dev):
-        _lib.check(_lib.lib().tk_kv8_append(
-            k3.data_ptr(), ks, v3.data_ptr(), vs, k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(),
-            tail.data_ptr(), nb, code, B, S, hkv, D, start_pos, _lib.dtype_code(k.dtype), _lib.stream_ptr(dev)),
-            "tk_kv8_append", 1 if B * S else 0)
+    launch(idx, "tk_kv8_append", 1 if B * S else 0, _lib.lib().tk_kv8_append, k.data_ptr(), ks, v.data_ptr(), vs,
+           k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), tail.data_ptr(), nb, code, B, S, hkv, D, start_pos,
+           _lib.dtype_code(k.dtype))
 
 
 def kv8_unpack(codes: torch.Tensor, values: bool, head_dim: int) -> torch.Tensor:
