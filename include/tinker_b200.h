@@ -251,7 +251,7 @@ TK_API int tk_beam_select(const void* logits, int64_t row_stride, const float* s
                           int64_t eos_token, float* out_scores, int64_t* out_beams, int64_t* out_tokens, int batch,
                           int beams, int vocab, int num_select, void* workspace, int64_t workspace_bytes, int dtype,
                           void* stream);
-TK_API int64_t tk_beam_select_workspace(int batch, int beams, int vocab, int num_select);
+TK_API int64_t tk_beam_select_workspace(int batch, int beams, int vocab, int num_select, int dtype);
 
 /*
  * Reorder a KV cache's rows in place after a beam search step: of each group of `beams` consecutive rows, row i

@@ -309,3 +309,34 @@ def test_reorder_odd_heads_errors_and_refusals():
     with pytest.raises(RuntimeError, match="32 beams"):
         kv_reorder(torch.zeros(33, 1, 4, 8, device="cuda").half(), torch.zeros(33, 1, 4, 8, device="cuda").half(),
                    torch.zeros(1, 33, dtype=torch.int64, device="cuda"), 2)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+def test_long_rows_that_stream(dt):
+    """Enough rows that a CTA's segment is longer than what it holds at once: masked beginnings, maxima anywhere, rising
+    and falling logits, references that prove too low, ties across the segment, NaN and +inf."""
+    require_b200()
+    dtype = DTYPES[dt]
+    B, K, V = 60, 10, 50021
+    g = torch.Generator(device="cuda").manual_seed(2)
+    logits = (torch.randn(B, K, V, device="cuda", generator=g) * 2).to(dtype)
+    scores = -torch.rand(B, K, device="cuda", generator=g) * 4
+    check(logits, scores, 20)
+    low = -math.inf if dt == "fp16" else torch.finfo(dtype).min
+    logits[0, :, :40000] = low                   # a masked beginning
+    logits[1] = low                              # nothing left
+    logits[2] = low
+    logits[2, 3, 49999] = 1.0                    # one token left, at the end
+    logits[3, :, 30000:] += 200                  # the maximum far above the first elements
+    logits[4, :, 30000:] -= 200
+    logits[5] = torch.linspace(-20, 20, V, device="cuda").to(dtype)   # rising: every element is a new maximum
+    logits[6] = torch.linspace(20, -20, V, device="cuda").to(dtype)
+    logits[7] = 1.5                              # all equal
+    logits[8, :, 9000:] = 3.0                    # thousands of equal ones behind the first elements
+    logits[9, 0, 45000] = math.nan
+    logits[10, 1, 45000] = math.inf
+    logits[11] = -1500.0                         # far below zero throughout
+    logits[12, :, :20000] = -600.0               # a plausible reference that is too low
+    check(logits, scores, 20)
+    check(logits[:, :, 1:], scores, 7)           # rows that start anywhere

@@ -78,7 +78,7 @@ SIGNATURES = {
                          _I, _I, _P, _I, _P, _I64, _I, _P],
     "tk_kv8_attention_workspace": [_I, _I, _I, _I, _I, _I],
     "tk_beam_select": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _P, _I64, _I, _P],
-    "tk_beam_select_workspace": [_I, _I, _I, _I],
+    "tk_beam_select_workspace": [_I, _I, _I, _I, _I],
     "tk_kv_reorder": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P],
     "tk_kv8_reorder": [_P, _P, _P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _P],
     "tk_decode_step_scratch_bytes": [_I, _I, _I, _I, _I, _I, _I, _I],

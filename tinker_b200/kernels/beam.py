@@ -17,9 +17,9 @@ from tinker_b200.kernels._common import launch
 
 
 @functools.lru_cache(maxsize=256)
-def _workspace_bytes(idx: int, batch: int, beams: int, vocab: int, num_select: int) -> int:
+def _workspace_bytes(idx: int, batch: int, beams: int, vocab: int, num_select: int, dtype: int) -> int:
     with torch.cuda.device(idx):
-        n = _lib.lib().tk_beam_select_workspace(batch, beams, vocab, num_select)
+        n = _lib.lib().tk_beam_select_workspace(batch, beams, vocab, num_select, dtype)
     if n < 0:
         raise RuntimeError(f"tk_beam_select_workspace: {_lib.last_error()}")
     return n
@@ -66,11 +66,11 @@ def beam_select(logits: torch.Tensor, scores: torch.Tensor, num_select: int | No
     tokens = torch.empty_like(beams)
     if B == 0:
         return out, beams, tokens
-    need = _workspace_bytes(idx, B, K, V, n)
+    dtype = _lib.dtype_code(logits.dtype)
+    need = _workspace_bytes(idx, B, K, V, n, dtype)
     ws = torch.empty(need, dtype=torch.uint8, device=out.device)
     launch(idx, "tk_beam_select", 2, _lib.lib().tk_beam_select, logits.data_ptr(), row, scores.data_ptr(), fin_ptr, eos,
-           out.data_ptr(), beams.data_ptr(), tokens.data_ptr(), B, K, V, n, ws.data_ptr(), need,
-           _lib.dtype_code(logits.dtype))
+           out.data_ptr(), beams.data_ptr(), tokens.data_ptr(), B, K, V, n, ws.data_ptr(), need, dtype)
     return out, beams, tokens
 
 
