@@ -131,11 +131,13 @@ struct ChunkSmem {
   float red[WARPS], red2[WARPS];
   uint32_t warp_key[WARPS];
   ulonglong2 box[WARPS];
-  uint32_t cand_key[CAP];
-  int cand_idx[CAP];
+  ulonglong2 cand2[CAP / 2];  // key << 32 | ~index: larger is better
   uint4 hit[HITS];
   int hit_at[HITS];
   int n_cand, n_hit;
+  __device__ uint64_t* cand() { return reinterpret_cast<uint64_t*>(cand2); }
+  __device__ float value(int i) { return value_of(static_cast<uint32_t>(cand()[i] >> 32)); }
+  __device__ int index(int i) { return static_cast<int>(~static_cast<uint32_t>(cand()[i])); }
 };
 
 // A segment in the plain way, element tid, tid + THREADS, ... for a thread.
@@ -184,28 +186,30 @@ __device__ __forceinline__ void plain_segment(const Params& p, const typename Lo
 // after the call. At least n candidates: the n-th value is the new threshold.
 __device__ __forceinline__ void rank_candidates(ChunkSmem& sm, int c, int n) {
   constexpr int EACH = CAP / THREADS;
-  uint32_t k[EACH];
-  int at[EACH], rank[EACH];
+  const int tid = threadIdx.x;
+  if (tid == 0 && (c & 1)) sm.cand()[c] = 0;  // read in pairs
+  __syncthreads();
+  uint64_t k[EACH];
+  int rank[EACH];
 #pragma unroll
   for (int e = 0; e < EACH; ++e) {
-    const int i = threadIdx.x + THREADS * e;
+    const int i = tid + THREADS * e;
     rank[e] = n;
     if (i < c) {
-      k[e] = sm.cand_key[i];
-      at[e] = sm.cand_idx[i];
+      k[e] = sm.cand()[i];
       rank[e] = 0;
 #pragma unroll 4
-      for (int o = 0; o < c; ++o) rank[e] += sm.cand_key[o] > k[e] || (sm.cand_key[o] == k[e] && sm.cand_idx[o] < at[e]);
+      for (int o = 0; 2 * o < c; ++o) {
+        const ulonglong2 x = sm.cand2[o];
+        rank[e] += (x.x > k[e]) + (x.y > k[e]);
+      }
     }
   }
   __syncthreads();
 #pragma unroll
   for (int e = 0; e < EACH; ++e)
-    if (rank[e] < n) {
-      sm.cand_key[rank[e]] = k[e];
-      sm.cand_idx[rank[e]] = at[e];
-    }
-  if (threadIdx.x == 0) sm.n_cand = min(c, n);
+    if (rank[e] < n) sm.cand()[rank[e]] = k[e];
+  if (tid == 0) sm.n_cand = min(c, n);
   __syncthreads();
 }
 
@@ -249,20 +253,28 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
       return fmaxf(fmaxf(get(v, 0), get(v, 1)), fmaxf(get(v, 2), get(v, 3))) > t;
     } else {
       const auto* w = reinterpret_cast<const typename Dt<DT>::T2*>(&v);
-      const auto t2 = Dt<DT>::pack(t, t);
-      return !(__hble2(w[0], t2) && __hble2(w[1], t2) && __hble2(w[2], t2) && __hble2(w[3], t2));
+      const float2 f = Dt<DT>::unpack(__hmax2(__hmax2(w[0], w[1]), __hmax2(w[2], w[3])));
+      return fmaxf(f.x, f.y) > t;
     }
   };
-  auto add = [&](float& sum, const uint4& v, float b) {
+  auto add = [&](float& sum, const uint4& v, float nb) {
+    const uint32_t w[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
-    for (int i = 0; i < VE; ++i) sum += exp2_approx(fmaf(get(v, i), L2E, -b));
+    for (int i = 0; i < 4; ++i) {
+      if constexpr (DT == TK_F32) {
+        sum += exp2_approx(fmaf(__uint_as_float(w[i]), L2E, nb));
+      } else {
+        float2 f;
+        if constexpr (DT == TK_BF16) f = make_float2(__uint_as_float(w[i] << 16), __uint_as_float(w[i] & 0xffff0000u));
+        else f = Dt<DT>::unpack(*reinterpret_cast<const typename Dt<DT>::T2*>(&w[i]));
+        sum += exp2_approx(fmaf(f.x, L2E, nb));
+        sum += exp2_approx(fmaf(f.y, L2E, nb));
+      }
+    }
   };
   auto push = [&](float x, int at) {
     const int slot = atomicAdd(&sm.n_cand, 1);
-    if (slot < CAP) {
-      sm.cand_key[slot] = key_of(x);
-      sm.cand_idx[slot] = at;
-    }
+    if (slot < CAP) sm.cand()[slot] = static_cast<uint64_t>(key_of(x)) << 32 | static_cast<uint32_t>(~at);
   };
   auto put_aside = [&](const uint4& v, int at) {
     const int slot = atomicAdd(&sm.n_hit, 1);
@@ -321,7 +333,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
   float sum = 0.f;
 #pragma unroll
   for (int j = 0; j < NV; ++j) {
-    add(sum, raw[j], b);
+    add(sum, raw[j], -b);
     asm volatile("" : "+f"(sum));  // a vector at a time: all converted at once would take twice the registers
   }
   if (mine > reach) {
@@ -368,30 +380,39 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
   if (!plain) rank_candidates(sm, sm.n_cand, p.n);
 
   if constexpr (STREAM) {
-    const int steps = (hi - lo + STEP - 1) / STEP;
+    const int steps = (hi - lo + STEP - 1) / STEP, full = aligned ? (hi - lo) / STEP : 0;
+    const uint4* from = reinterpret_cast<const uint4*>(src + lo) + tid;
 #pragma unroll 1
     for (int it = NV; it < steps && !plain;) {
       __syncthreads();  // the counters of the last round have been read
       if (tid == 0) sm.n_hit = 0;
-      const float t = value_of(sm.cand_key[p.n - 1]);
+      const float t = sm.value(p.n - 1);
       __syncthreads();
       const int stop = min(steps, it + STRIDE);
+      const float nb = -b;
 #pragma unroll 1
       for (; it < stop; it += 2) {
+        uint4 v[2];
+#pragma unroll
+        for (int e = 0; e < 2; ++e) v[e] = ahead[e];
+        if (it + 3 < full) {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) ahead[e] = __ldcs(from + (it + 2 + e) * THREADS);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 2; ++e) ahead[e] = load(static_cast<int64_t>(lo) + STEP * (it + 2 + e) + tid * VE);
+        }
 #pragma unroll
         for (int e = 0; e < 2; ++e) {  // what is behind the segment is -inf and adds nothing
-          const uint4 v = ahead[e];
-          const int at = lo + STEP * (it + e) + tid * VE;
-          ahead[e] = load(static_cast<int64_t>(at) + 2 * STEP);
-          if (exceeds(v, t)) put_aside(v, at);
-          add(sum, v, b);
+          if (exceeds(v[e], t)) put_aside(v[e], lo + STEP * (it + e) + tid * VE);
+          add(sum, v[e], nb);
         }
       }
       sift(t);
       plain = sm.n_hit > HITS || sm.n_cand > CAP;
       if (plain || sm.n_cand == p.n) continue;
       rank_candidates(sm, sm.n_cand, p.n);
-      const float best = value_of(sm.cand_key[0]);
+      const float best = sm.value(0);
       if (best > ref + 16.f && best < INFINITY) {  // far above the reference: the sum goes by it from here on
         const float nb = best * L2E;
         sum *= exp2_approx(b - nb);
@@ -413,7 +434,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
     return v;
   };
   sum = total(sum);
-  const float best = sm.n_cand > 0 && !plain ? value_of(sm.cand_key[0]) : INFINITY;
+  const float best = sm.n_cand > 0 && !plain ? sm.value(0) : INFINITY;
   if (plain || !(sum <= INFINITY) || !(best < INFINITY)) {  // the second is true of NaN
     plain_segment<DT>(p, src, lo, hi, part, sm);
     return;
@@ -436,7 +457,7 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
   if (tid == 0) p.part_ms[part] = make_float2(ref, sum);
   Entry* top = p.part_top + part * p.n;
   for (int i = tid; i < p.n; i += THREADS)  // a segment shorter than n has fewer
-    top[i] = i < sm.n_cand ? Entry{value_of(sm.cand_key[i]), sm.cand_idx[i]} : Entry{-INFINITY, -1};
+    top[i] = i < sm.n_cand ? Entry{sm.value(i), sm.index(i)} : Entry{-INFINITY, -1};
 }
 
 // Candidate j of a still beam: the end token of a finished one first, then -inf at its lowest tokens.
