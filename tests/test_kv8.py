@@ -9,6 +9,10 @@ from the data of each case: with S1 = max sum |q k| / sqrt(D), n keys and a 16-b
 The score of a key carries the split's remainder (2^-22 |q k|) and D + 8 roundings of fp32 sums; a weight's relative
 error is that of the score on both sides of the quotient (twice, and twice for max - score), the exponential and the
 split of the weight add less than 2^-20, the fp32 sum over n keys at most n 2^-24.
+
+From 64 query rows of a kv head on, at a position known on the host, q and the weights are rounded to f16 once: 2^-12 of
+each of a score's terms (so 2^-12 S1 of a score, twice for the quotient) and 2^-12 of a weight. The bound then has
+2 max|v| (2^-11 S1 + 2^-12) more.
 """
 
 import math
@@ -63,9 +67,10 @@ def make_cache(B, hkv, d, cap, starts, dtype, code, gen, garbage=True):
     return kc, vc, sc, tail, rows
 
 
-def exact(q, k, v, cos, sin, rows, starts, hq, hkv, d):
+def exact(q, k, v, cos, sin, rows, starts, hq, hkv, d, on_host=True):
     """64-bit rows of the attention and each element's bound."""
     B, S = q.shape[:2]
+    once = on_host and hq // hkv * S >= 64
     dtype, g = q.dtype, hq // hkv
     st = torch.tensor(starts, device="cuda")
     q4, k4 = q.double().reshape(B, S, hq, d), k.float().reshape(B, S, hkv, d)
@@ -87,7 +92,7 @@ def exact(q, k, v, cos, sin, rows, starts, hq, hkv, d):
             o = torch.softmax(s.masked_fill(future, -math.inf), -1) @ V
             out[b, :, h] = o
             tol[b, :, h] = torch.finfo(dtype).eps / 2 * o.abs() + 2 * V.abs().max() * (
-                4 * (d + 8) * 2.0 ** -24 * s1 + n * 2.0 ** -24 + 2.0 ** -20)
+                4 * (d + 8) * 2.0 ** -24 * s1 + n * 2.0 ** -24 + 2.0 ** -20 + once * (2.0 ** -11 * s1 + 2.0 ** -12))
     return out.reshape(B, S, hq * d), tol.reshape(B, S, hq * d), k4.to(dtype), v4.to(dtype)
 
 
@@ -298,6 +303,14 @@ ATTENTION = [  # dt, code, B, hq, hkv, d, starts, S
     ("bf16", "e4m3", 1, 4, 4, 128, [64], 64),
     ("fp16", "int8", 1, 16, 4, 64, [1025], 257),
     ("fp16", "e4m3", 3, 8, 2, 64, [0, 45, 400], 35),     # chunks at positions of their own
+    # the tensor-core form: one query tile or two, an odd number of pairs, keys split or not, tiles that end anywhere
+    ("bf16", "e4m3", 1, 32, 8, 128, [2000], 130),
+    ("fp16", "int8", 2, 16, 4, 64, [128, 128], 96),
+    ("bf16", "int8", 1, 14, 2, 64, [5000], 150),
+    ("bf16", "e4m3", 5, 32, 8, 64, [63] * 5, 200),
+    ("fp16", "e4m3", 1, 8, 4, 128, [0], 300),
+    ("bf16", "int8", 1, 16, 1, 128, [127], 33),
+    ("fp16", "e4m3", 2, 4, 4, 64, [1000, 1000], 128),
 ]
 
 
@@ -318,7 +331,7 @@ def test_attention(dt, code, B, hq, hkv, d, starts, S, tables):
     cos = sin = None
     if tables:
         cos, sin = precompute_rope_tables(d, cap, 1e4, device="cuda")
-    want, tol, k_new, v_new = exact(q, k, v, cos, sin, rows, starts, hq, hkv, d)
+    want, tol, k_new, v_new = exact(q, k, v, cos, sin, rows, starts, hq, hkv, d, on_host=len(set(starts)) == 1)
     after = [t.clone() for t in (kc, vc, sc, tail)]
     for b in range(B):
         kv8_append(k_new[b:b + 1].reshape(1, S, -1), v_new[b:b + 1].reshape(1, S, -1), *(t[b:b + 1] for t in after),

@@ -84,6 +84,14 @@ __device__ __forceinline__ float block_scale(uint32_t amax_bits, float& inv) {
   return fine ? __fdiv_rn(a, Code<FMT>::LIMIT) : __uint_as_float(0x7fc00000u);
 }
 
+// The power of two, at most 2^60, that brings `amax` (fp32 bits of a magnitude) to [2^14, 2^15); 1 if it is not finite.
+// (A tile of zeros has the inverse of the factor as its scale, and sums of that have to stay finite.)
+__device__ __forceinline__ float to_f16_range(uint32_t amax_bits) {
+  const int e = static_cast<int>(amax_bits >> 23);
+  if (e >= 255) return 1.f;
+  return __uint_as_float(static_cast<uint32_t>(min(187, 268 - e)) << 23);
+}
+
 template <int DT>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return Dt<DT>::unpack(*reinterpret_cast<const typename Dt<DT>::T2*>(&w));

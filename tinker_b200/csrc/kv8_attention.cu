@@ -30,7 +30,8 @@
 // A warp copies its tiles ahead into a ring of its own in shared memory (cp.async), and the first tiles of its next
 // unit before it puts the last one's rows away. For S = 1 the warp that holds the open block also appends the row, or
 // encodes the block if the row completes it (nothing in the launch reads that block from the cache); for S > 1 a
-// second launch appends, since other warps still read the tail.
+// second launch appends, since other warps still read the tail. Many rows at a position known on the host take
+// kv8_chunk.cu.
 #include <algorithm>
 #include <string>
 #include <type_traits>
@@ -104,13 +105,6 @@ __device__ __forceinline__ void split2(float x, float y, uint32_t& hi, uint32_t&
   const float2 f = __half22float2(h);
   hi = h2_u32(h);
   lo = h2_u32(__floats2half2_rn(x - f.x, y - f.y));
-}
-
-// The power of two that brings `amax` (fp32 bits of a magnitude) to [2^14, 2^15); 1 if it is not finite.
-__device__ __forceinline__ float to_f16_range(uint32_t amax_bits) {
-  const int e = static_cast<int>(amax_bits >> 23);
-  if (e >= 255) return 1.f;
-  return __uint_as_float(static_cast<uint32_t>(min(254, 268 - e)) << 23);
 }
 
 // 8 x 8 16-bit matrix transposed: lane 4i + q gives row i, columns 2q and 2q + 1, and takes them of the transpose.
@@ -858,6 +852,7 @@ int64_t parts_bytes(int sm_count) {
   return int64_t(Smem<D, NG>::CTAS_SM) * sm_count * 2 * Smem<D, NG>::PART;
 }
 int64_t workspace_bytes_for(int head_dim, int sm_count) {
+  sm_count = std::max(sm_count, 1);
   return counter_bytes(sm_count) + (head_dim == 64 ? std::max(parts_bytes<64, 1>(sm_count), parts_bytes<64, 2>(sm_count))
                                                    : std::max(parts_bytes<128, 1>(sm_count), parts_bytes<128, 2>(sm_count)));
 }
@@ -912,7 +907,10 @@ extern "C" int64_t tk_kv8_attention_workspace(int batch, int num_heads, int num_
     return 0;
   DeviceInfo di;
   if (current_device_info(&di)) return -1;
-  return kv8::workspace_bytes_for(head_dim, di.sm_count);
+  int64_t need = kv8::workspace_bytes_for(head_dim, di.sm_count);
+  if (kv8::chunk_fits(batch, num_heads, num_kv_heads, seq, max_kv))
+    need += kv8::chunk_workspace(batch, num_heads, num_kv_heads, head_dim, seq, max_kv, di.sm_count);
+  return need;
 }
 
 extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
@@ -951,9 +949,24 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   if (int rc = current_device_info(&di)) return rc;
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
   if (rows > INT32_MAX) return fail_invalid("kv8_attention: too many query rows for one call");
-  if (!workspace || workspace_bytes < workspace_bytes_for(head_dim, di.sm_count))
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t small = workspace_bytes_for(head_dim, di.sm_count);
+  // with the position in device memory the length, and so the tiles, are not known here
+  const bool chunk = !start_pos_device && chunk_fits(batch, num_heads, num_kv_heads, seq, int64_t(start_pos) + seq);
+  const int64_t need = small + (chunk ? chunk_workspace(batch, num_heads, num_kv_heads, head_dim, seq,
+                                                        int64_t(start_pos) + seq, di.sm_count) : 0);
+  if (!workspace || workspace_bytes < need)
     return fail_invalid("kv8_attention: workspace missing or smaller than tk_kv8_attention_workspace()");
   if (!aligned16(workspace)) return fail_invalid("kv8_attention: workspace must be 16-byte aligned");
+  if (chunk) {
+    // behind the counters and parts of the other form, which have to stay as they are
+    if (int rc = chunk_attention(c, q, q_tok_stride, k, k_tok_stride, v, v_tok_stride, cos_table, sin_table, out,
+                                 out_tok_stride, batch, seq, num_heads, num_kv_heads, head_dim, start_pos,
+                                 static_cast<char*>(workspace) + small, dtype, di.sm_count, st))
+      return rc;
+    return append(c, k, k_tok_stride, v, v_tok_stride, cos_table, sin_table, table_rows, batch, seq, num_kv_heads,
+                  head_dim, start_pos, nullptr, 0, dtype, st);
+  }
   AttnParams p{};
   p.q = q;
   p.qs = q_tok_stride;
@@ -980,7 +993,6 @@ extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void*
   p.start_step = start_pos_step;
   p.batch = batch;
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
   int rc;
   if (dtype == TK_F16)
     rc = format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, head_dim, workspace, di, st)

@@ -63,11 +63,11 @@ def kv8_attention_workspace(batch: int, num_heads: int, num_kv_heads: int, head_
     return int(n)
 
 
-@functools.lru_cache(maxsize=64)
-def _workspace_bytes(idx: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
-    """``kv8_attention_workspace`` on device ``idx``; the size does not depend on the other arguments."""
+@functools.lru_cache(maxsize=256)
+def _workspace_bytes(idx: int, *sizes) -> int:
+    """``kv8_attention_workspace`` on device ``idx``."""
     with torch.cuda.device(idx):
-        return kv8_attention_workspace(1, num_heads, num_kv_heads, head_dim, 1, 1)
+        return kv8_attention_workspace(*sizes)
 
 
 def _rows(t: torch.Tensor, B: int, S: int, width: int) -> tuple[torch.Tensor, int]:
@@ -158,7 +158,10 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
     out = q.new_empty((B, S, width))
     if B == 0 or S == 0:
         return out
-    need = _workspace_bytes(idx, num_heads, num_kv_heads, head_dim)
+    if S == 1 or pos_ptr is not None:  # independent of the other sizes
+        need = _workspace_bytes(idx, 1, num_heads, num_kv_heads, head_dim, 1, 1)
+    else:
+        need = _workspace_bytes(idx, B, num_heads, num_kv_heads, head_dim, S, start_pos + S)
     if workspace is None:
         workspace = torch.zeros(need, dtype=torch.uint8, device=out.device)
     elif workspace.nbytes < need or workspace.get_device() != idx or not workspace.is_contiguous():
