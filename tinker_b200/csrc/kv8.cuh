@@ -155,9 +155,10 @@ __device__ __forceinline__ void rope_chunk(uint4& x, const float* cos_row, const
   }
 }
 
-// Quantise a block of keys: `piece(token, c)` gives 16-byte chunk c of a token's row. One warp; returns the scale.
-template <int DT, int FMT, int D, typename F>
-__device__ __forceinline__ float encode_keys(uint8_t* block, int lane, F piece) {
+// Quantise a block of keys: `piece(token, c)` loads 16-byte chunk c of a token's row, `finish(x, token, c)` completes it
+// when all loads are on their way. One warp; returns the scale.
+template <int DT, int FMT, int D, typename F, typename G>
+__device__ __forceinline__ float encode_keys(uint8_t* block, int lane, F piece, G finish) {
   constexpr int H = D / 64;
   const int n = lane >> 2, q = lane & 3;
   uint4 x[4][H][2];
@@ -173,8 +174,10 @@ __device__ __forceinline__ float encode_keys(uint8_t* block, int lane, F piece) 
 #pragma unroll
     for (int h = 0; h < H; ++h)
 #pragma unroll
-      for (int e = 0; e < 2; ++e)
+      for (int e = 0; e < 2; ++e) {
+        finish(x[j][h][e], 8 * (n >> 1) + 2 * j + (n & 1), 8 * h + 2 * q + e);
         m = amax2(amax2(amax2(amax2(m, x[j][h][e].x), x[j][h][e].y), x[j][h][e].z), x[j][h][e].w);
+      }
   float inv;
   const float scale = block_scale<DT, FMT>(amax2_warp(m), inv);
 #pragma unroll

@@ -65,32 +65,37 @@ __global__ void __launch_bounds__(PAIRS * 64) kv8_append_kernel(const AppendPara
   const int row0 = task * BLOCK - open;  // the input row of the block's first token
   // 16-byte chunk c of input row s, rotated if it is a key
   auto fresh = [&](int s, int c) {
-    uint4 x = __ldcg(reinterpret_cast<const uint4*>(in + (static_cast<int64_t>(b) * p.seq + s) * stride) + c);
-    if (!values && p.cos_t) {
+    return __ldcg(reinterpret_cast<const uint4*>(in + (static_cast<int64_t>(b) * p.seq + s) * stride) + c);
+  };
+  auto rotate = [&](uint4& x, int s, int c) {
+    if (!values && p.cos_t && s >= 0) {
       const int64_t at = (static_cast<int64_t>(start) + s) * (D / 2) + c * 4;
       rope_chunk<DT>(x, p.cos_t + at, p.sin_t + at);
     }
-    return x;
   };
-  auto piece = [&](int t, int c) {
-    if (row0 + t < 0) return __ldcg(reinterpret_cast<const uint4*>(tail + t * D) + c);
-    return fresh(row0 + t, c);
+  auto piece = [&](int t, int c) {  // one load whatever its source, so that a lane's loads are all in flight at once
+    const int s = row0 + t;
+    const T* src = s < 0 ? tail + t * D : in + (static_cast<int64_t>(b) * p.seq + s) * stride;
+    return __ldcg(reinterpret_cast<const uint4*>(src) + c);
   };
 
   if (whole > 0) {
     const int64_t block = bh * p.num_blocks + first + task;
     float scale;
     if (!values) {
-      scale = encode_keys<DT, FMT, D>(p.kc + block * (BLOCK * D), lane, piece);
+      scale = encode_keys<DT, FMT, D>(p.kc + block * (BLOCK * D), lane, piece,
+                                       [&](uint4& x, int t, int c) { rotate(x, row0 + t, c); });
     } else {
       uint8_t* tile = smem + (warp - PAIRS) * (BLOCK * D * 2);
       uint32_t m = 0;
+      uint4 x[C16];
+#pragma unroll
+      for (int i = 0; i < C16; ++i) x[i] = piece((lane + 32 * i) / C16, (lane + 32 * i) % C16);
 #pragma unroll
       for (int i = 0; i < C16; ++i) {
         const int idx = lane + 32 * i, t = idx / C16, c = idx % C16;
-        const uint4 x = piece(t, c);
-        m = amax2(amax2(amax2(amax2(m, x.x), x.y), x.z), x.w);
-        *reinterpret_cast<uint4*>(tile + tile_off<D>(t, c)) = x;
+        m = amax2(amax2(amax2(amax2(m, x[i].x), x[i].y), x[i].z), x[i].w);
+        *reinterpret_cast<uint4*>(tile + tile_off<D>(t, c)) = x[i];
       }
       const uint32_t amax = amax2_warp(m);
       __syncwarp();
@@ -102,7 +107,9 @@ __global__ void __launch_bounds__(PAIRS * 64) kv8_append_kernel(const AppendPara
     const int n = whole > 0 ? rest : p.seq, to = whole > 0 ? 0 : open, from = p.seq - n;
     for (int idx = lane; idx < n * C16; idx += 32) {
       const int t = idx / C16, c = idx % C16;
-      *(reinterpret_cast<uint4*>(tail + (to + t) * D) + c) = fresh(from + t, c);
+      uint4 x = fresh(from + t, c);
+      rotate(x, from + t, c);
+      *(reinterpret_cast<uint4*>(tail + (to + t) * D) + c) = x;
     }
   }
 }

@@ -645,7 +645,7 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
           const int64_t block = bh * p.num_blocks + n8;
           const float sk = encode_keys<DT, FMT, D>(p.kc + block * S::HALF, lane, [&](int tok, int c) {
             return *reinterpret_cast<const uint4*>(ktile + tile_off<D>(tok, c));
-          });
+          }, [](uint4&, int, int) {});
           const float sv = encode_values<DT, FMT, D>(p.vc + block * S::HALF, lane, smem_u32(vtile), vm);
           if (lane == 0) reinterpret_cast<float2*>(p.scales)[block] = make_float2(sk, sv);
         }

@@ -202,21 +202,22 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) kv8_expand_kernel(const Par
   const int row0 = (block - n8) * BLOCK - open;  // the call's row of the block's first token
   uint8_t* tile = smem + warp * (BLOCK * D * 2);
   uint32_t m = 0;
-#pragma unroll 4
+  uint4 x[C16];
+#pragma unroll
+  for (int i = 0; i < C16; ++i) {  // all loads in flight, then the rotations
+    const int idx = lane + 32 * i, t = idx / C16, c = idx % C16, s = row0 + t;
+    const T* src = s < 0 ? tail + t * D : in + (static_cast<int64_t>(b) * p.seq + min(s, p.seq - 1)) * stride;
+    x[i] = s < p.seq ? __ldcg(reinterpret_cast<const uint4*>(src) + c) : make_uint4(0, 0, 0, 0);
+  }
+#pragma unroll
   for (int i = 0; i < C16; ++i) {
     const int idx = lane + 32 * i, t = idx / C16, c = idx % C16, s = row0 + t;
-    uint4 x = make_uint4(0, 0, 0, 0);
-    if (s < 0) {
-      x = __ldcg(reinterpret_cast<const uint4*>(tail + t * D) + c);
-    } else if (s < p.seq) {
-      x = __ldcg(reinterpret_cast<const uint4*>(in + (static_cast<int64_t>(b) * p.seq + s) * stride) + c);
-      if (!values && p.cos_t) {
-        const int64_t ang = (static_cast<int64_t>(p.start) + s) * (D / 2) + c * 4;
-        rope_chunk<DT>(x, p.cos_t + ang, p.sin_t + ang);
-      }
+    if (!values && p.cos_t && s >= 0 && s < p.seq) {
+      const int64_t ang = (static_cast<int64_t>(p.start) + s) * (D / 2) + c * 4;
+      rope_chunk<DT>(x[i], p.cos_t + ang, p.sin_t + ang);
     }
-    m = amax2(amax2(amax2(amax2(m, x.x), x.y), x.z), x.w);
-    *reinterpret_cast<uint4*>(tile + tile_off<D>(t, c)) = x;
+    m = amax2(amax2(amax2(amax2(m, x[i].x), x[i].y), x[i].z), x[i].w);
+    *reinterpret_cast<uint4*>(tile + tile_off<D>(t, c)) = x[i];
   }
   const uint32_t amax = amax2_warp(m);
   __syncwarp();
@@ -423,9 +424,10 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int first_pos = p.start + (2 * pair + x) * BQ / p.groups;  // of the tile's first row: keys to there are open
       const float4* sx = p.sx + bh * (p.keys / BLOCK) + static_cast<int64_t>(lo) * (BKV / BLOCK);
       for (int j = 0; ok && j < n_x; ++j) {
-        float4 sc[4];
+        float4 sc[4];  // from L1: one line holds two tiles' and the line after it is on its way
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = __ldcg(sx + 4 * j + i);
+        for (int i = 0; i < 4; ++i) sc[i] = sx[4 * j + i];
+        if (lane == 0 && j + 3 < n_x) prefetch_l1(sx + 4 * (j + 3));
         if (!mbar_wait(bars + B_S_FULL + x, j & 1)) { ok = false; break; }
         tc_fence_after();
         float sv[BKV];
@@ -556,14 +558,24 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Params p) {
   const int64_t bh = static_cast<int64_t>(blockIdx.z) * p.num_kv_heads + blockIdx.y;
   const int64_t slot = (bh * p.rows + row) * p.splits;
   float M = -INFINITY, L = 0.f, acc[E] = {};
+  const float* from = p.part_o + slot * D + lane * E;
   for (int i = 0; i < p.splits; ++i) {
     const float2 ml = __ldcg(p.part_ml + slot + i);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key of this row in the part
     const float mn = fmaxf(M, ml.x);
     const float a = exp2_approx(M - mn), e = exp2_approx(ml.x - mn);
     L = L * a + ml.y * e;
-#pragma unroll
-    for (int c = 0; c < E; ++c) acc[c] = acc[c] * a + __ldcg(p.part_o + (slot + i) * D + lane * E + c) * e;
+    if constexpr (E == 4) {
+      const float4 o = __ldcg(reinterpret_cast<const float4*>(from + static_cast<int64_t>(i) * D));
+      acc[0] = acc[0] * a + o.x * e;
+      acc[1] = acc[1] * a + o.y * e;
+      acc[2] = acc[2] * a + o.z * e;
+      acc[3] = acc[3] * a + o.w * e;
+    } else {
+      const float2 o = __ldcg(reinterpret_cast<const float2*>(from + static_cast<int64_t>(i) * D));
+      acc[0] = acc[0] * a + o.x * e;
+      acc[1] = acc[1] * a + o.y * e;
+    }
     M = mn;
   }
   const float inv = 1.f / L;
