@@ -38,7 +38,8 @@ template <> struct Code<TK_KV8_INT8> {
 __device__ __forceinline__ uint32_t h2_u32(__half2 v) { return *reinterpret_cast<const uint32_t*>(&v); }
 __device__ __forceinline__ __half2 u32_h2(uint32_t v) { return *reinterpret_cast<const __half2*>(&v); }
 
-// Codes of four values, lowest byte first.
+// Codes of four values, lowest byte first. int8: 1.5 * 2^23 + v has v, rounded to even, in its low byte, in two's
+// complement (a conversion runs at a quarter of the rate: 16 x 4001 rows of 8 heads of 128 took 85.5 us, now 75.2).
 template <int FMT>
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) {
   if constexpr (FMT == TK_KV8_E4M3) {
@@ -47,8 +48,10 @@ __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d) 
     asm("cvt.rn.satfinite.e4m3x2.f32 %0, %1, %2;" : "=h"(hi) : "f"(d), "f"(c));
     return static_cast<uint32_t>(lo) | (static_cast<uint32_t>(hi) << 16);
   } else {
-    const int i0 = __float2int_rn(a), i1 = __float2int_rn(b), i2 = __float2int_rn(c), i3 = __float2int_rn(d);
-    return (i0 & 0xff) | ((i1 & 0xff) << 8) | ((i2 & 0xff) << 16) | (static_cast<uint32_t>(i3) << 24);
+    constexpr float MAGIC = 12582912.f;
+    const uint32_t lo = __byte_perm(__float_as_uint(__fadd_rn(a, MAGIC)), __float_as_uint(__fadd_rn(b, MAGIC)), 0x0040);
+    const uint32_t hi = __byte_perm(__float_as_uint(__fadd_rn(c, MAGIC)), __float_as_uint(__fadd_rn(d, MAGIC)), 0x0040);
+    return __byte_perm(lo, hi, 0x5410);
   }
 }
 
