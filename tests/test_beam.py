@@ -340,3 +340,24 @@ def test_long_rows_that_stream(dt):
     logits[12, :, :20000] = -600.0               # a plausible reference that is too low
     check(logits, scores, 20)
     check(logits[:, :, 1:], scores, 7)           # rows that start anywhere
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["fp16", "bf16", "fp32"])
+@pytest.mark.parametrize("V, n", [(2300, 64), (2049, 8), (4500, 40), (33000, 64), (9000, 64)])
+def test_short_last_chunks_and_scattered_masks(V, n, dt):
+    """Chunks that end after a few elements, and rows of which a few stretches are not masked, so that the threads'
+    maxima say little about the n-th best."""
+    require_b200()
+    dtype = DTYPES[dt]
+    g = torch.Generator(device="cuda").manual_seed(V)
+    logits = (torch.randn(2, 3, V, device="cuda", generator=g) * 3).to(dtype)
+    scores = torch.tensor([[0.0, -0.5, -1.0], [-1.0, 0.0, -9.0]], device="cuda")
+    check(logits, scores, n)
+    low = -math.inf if dt != "bf16" else torch.finfo(dtype).min
+    masked = torch.full_like(logits, low)
+    for at in (0, 700, 1500, V - 30):
+        masked[:, :, at:at + 300] = logits[:, :, at:at + 300]
+    masked[0, 1] = low
+    masked[0, 1, 100:103] = 1.0
+    check(masked, scores, n)

@@ -92,20 +92,24 @@ __device__ __forceinline__ bool is_still(const Params& p, int row) {
   return done || !(score > -INFINITY);
 }
 
-// A key that at least n of the threads' keys reach, for n <= 8 * 32: see the head of this file. All threads call it.
-__device__ __forceinline__ uint32_t reach_of(uint32_t mine, int n, uint32_t* warp_key) {
+// A key that at least n of the keys of the first `warps` warps' threads reach (0 if there are too few of them): see the
+// head of this file. All threads call it.
+__device__ __forceinline__ uint32_t reach_of(uint32_t mine, int n, int warps, uint32_t* warp_key) {
   const int lane = threadIdx.x & 31;
   uint32_t left = mine, kth = 0;
-  for (int i = 0; i < (n + WARPS - 1) / WARPS; ++i) {
+  const int rounds = warps > 0 ? (n + warps - 1) / warps : 33;
+  for (int i = 0; i < min(rounds, 32); ++i) {
     kth = __reduce_max_sync(0xffffffffu, left);
     const uint32_t who = __ballot_sync(0xffffffffu, left == kth);
     if (lane == __ffs(who) - 1) left = 0;
   }
   if (lane == 0) warp_key[threadIdx.x >> 5] = kth;
   __syncthreads();
+  if (rounds > 32) return 0;
   uint32_t t = warp_key[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) t = min(t, warp_key[w]);
+  for (int w = 1; w < WARPS; ++w)
+    if (w < warps) t = min(t, warp_key[w]);
   return t;
 }
 
@@ -324,7 +328,9 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
   if (lane == 0) sm.red[warp] = mx;
-  float reach = value_of(reach_of(key_of(mine), p.n, sm.warp_key));  // synchronises
+  constexpr uint32_t LOWEST = 0x007fffffu;  // the key of -inf
+  const int warps = min(WARPS, (hi - lo) / (32 * VE));  // those whose threads all have elements of their own
+  float reach = value_of(max(reach_of(key_of(mine), p.n, warps, sm.warp_key), LOWEST));  // synchronises
   mx = sm.red[0];
 #pragma unroll
   for (int w = 1; w < WARPS; ++w) mx = fmaxf(mx, sm.red[w]);
@@ -336,14 +342,44 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
     add(sum, raw[j], -b);
     asm volatile("" : "+f"(sum));  // a vector at a time: all converted at once would take twice the registers
   }
-  if (mine > reach) {
+  auto collect = [&]() {
+    if (mine > reach) {
 #pragma unroll
-    for (int j = 0; j < NV; ++j)
-      if (exceeds(raw[j], reach)) put_aside(raw[j], lo + STEP * j + tid * VE);
+      for (int j = 0; j < NV; ++j)
+        if (exceeds(raw[j], reach)) put_aside(raw[j], lo + STEP * j + tid * VE);
+    }
+    sift(reach);
+  };
+  collect();
+  if (sm.n_hit > HITS || sm.n_cand > CAP) {
+    // the best elements lie in few threads' hands (most of the vocabulary is masked): the n-th largest value itself,
+    // bit by bit
+    uint32_t t = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const uint32_t probe = t | 1u << bit;
+      int count = 0;
+#pragma unroll
+      for (int j = 0; j < NV; ++j)
+#pragma unroll
+        for (int i = 0; i < VE; ++i) count += key_of(get(raw[j], i)) >= probe && lo + STEP * j + tid * VE + i < hi;
+      count = __reduce_add_sync(0xffffffffu, count);
+      __syncthreads();
+      if (lane == 0) sm.warp_key[warp] = count;
+      __syncthreads();
+      count = 0;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) count += static_cast<int>(sm.warp_key[w]);
+      if (count >= p.n) t = probe;
+    }
+    reach = value_of(max(t, LOWEST));
+    __syncthreads();
+    if (tid == 0) sm.n_cand = sm.n_hit = 0;
+    __syncthreads();
+    collect();
   }
-  sift(reach);
   const int above = sm.n_cand;
-  bool plain = sm.n_hit > HITS;
+  bool plain = sm.n_hit > HITS;  // a NaN at most
   __syncthreads();
   if (above < p.n && !plain) {  // equal ones in order of index: vector by vector, thread by thread
     int need = p.n - above;
@@ -558,8 +594,18 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const Params p) {
 #pragma unroll
   for (int e = 0; e < FIRST; ++e)
     if (THREADS * e < total) look(min(tid + THREADS * e, total - 1), raw[e]);
-  for (int i = tid + THREADS * FIRST; i < total; i += THREADS) look(i, load(i));
-  const uint32_t reach = max(reach_of(mine, p.n, warp_key), 1u);
+  for (int i0 = THREADS * FIRST; i0 < total; i0 += THREADS * FIRST) {  // as many at a time, all loads in flight
+    int2 more[FIRST];
+#pragma unroll
+    for (int e = 0; e < FIRST; ++e) {
+      const int i = i0 + tid + THREADS * e;
+      more[e] = i < total ? load(i) : make_int2(0, -1);
+    }
+#pragma unroll
+    for (int e = 0; e < FIRST; ++e)
+      if (i0 + THREADS * e < total) look(min(i0 + tid + THREADS * e, total - 1), more[e]);
+  }
+  const uint32_t reach = max(reach_of(mine, p.n, WARPS, warp_key), 1u);
   auto keep = [&](int i, int2 t) {
     double c;
     uint64_t at;
@@ -574,6 +620,7 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const Params p) {
 #pragma unroll
     for (int e = 0; e < FIRST; ++e)
       if (tid + THREADS * e < total) keep(tid + THREADS * e, raw[e]);
+#pragma unroll 4
     for (int i = tid + THREADS * FIRST; i < total; i += THREADS) keep(i, load(i));
   }
   __syncthreads();
@@ -598,7 +645,7 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const Params p) {
       }
       __syncthreads();
       if (tid == 0) n_cand = 0;
-      const uint32_t high = max(reach_of(best, p.n, warp_key), 1u);
+      const uint32_t high = max(reach_of(best, p.n, WARPS, warp_key), 1u);
 #pragma unroll
       for (int e = 0; e < CAP / THREADS; ++e)
         if (k[e] >> 32 >= high) {
