@@ -519,3 +519,21 @@ def test_other_stream_repeat_and_refusals():
         kv8_attention(q, k.half(), v, cos, sin, *args, start_pos=n)
     with pytest.raises(ValueError, match="capacity"):
         kv8_append(k, v, kc, vc, sc, tail, kc.shape[2] * 32)
+
+
+@pytest.mark.gpu
+def test_chunk_of_more_sequences_than_are_laid_out_at_once():
+    """Operands of all sequences would take more than the gigabyte that the call allows itself: it goes in groups."""
+    require_b200()
+    from tinker_b200.kernels import kv8_attention, kv8_attention_workspace
+    B, hq, hkv, d, n, S = 16, 32, 8, 128, 20000, 16
+    one = kv8_attention_workspace(1, hq, hkv, d, S, n + S) - kv8_attention_workspace(1, hq, hkv, d, 1, 1)
+    assert B * one > 2 ** 30
+    g = torch.Generator(device="cuda").manual_seed(4)
+    kc, vc, sc, tail, rows = make_cache(B, hkv, d, n + S, [n] * B, torch.bfloat16, "e4m3", g, garbage=False)
+    w = torch.randn(B, S, (hq + 2 * hkv) * d, device="cuda", generator=g).bfloat16()
+    q, k, v = w.split([hq * d, hkv * d, hkv * d], -1)
+    out = kv8_attention(q, k, v, None, None, kc, vc, sc, tail, hq, hkv, d, start_pos=n)
+    for b in (0, 7, 12, 13, 15):
+        want, tol, _, _ = exact(q[b:b + 1], k[b:b + 1], v[b:b + 1], None, None, rows[b:b + 1], [n], hq, hkv, d)
+        assert ((out[b:b + 1].double() - want).abs() <= tol).all(), b

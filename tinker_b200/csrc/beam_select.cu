@@ -688,7 +688,7 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const Params p) {
 // Vectors that a thread keeps in registers and the segment of a CTA. Segments of 1, 2 or 4 vectors a thread (8 to 32
 // 16-bit logits) where that gives up to two CTAs for every SM: 4 rows of 32000 make 64 CTAs of 2048 elements. More work
 // streams: segments of equal length, as many as it takes to fill the four CTAs that an SM holds once (256 rows of
-// 151936: 3 segments each, 49 us with 10 segments in registers, NN us streamed).
+// 151936: 3 segments each, 49 us with 10 segments in registers, 28 us streamed).
 struct Plan {
   int vectors, splits, segment;
   bool stream;

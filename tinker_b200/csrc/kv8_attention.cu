@@ -17,7 +17,7 @@
 //     denominator is sum w / scale_v. So O needs no pass per block, w stays in [0, 1], and the rounding of log2
 //     scale_v cancels between numerator and denominator.
 // (The keys as columns, with f16(q) and remainder as two halves of the 16 rows, took 274 instead of some 170
-// instructions for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 17 us for 64
+// instructions for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 18.8 us for 64
 // sequences of 4 kv heads at 2047.)
 //
 // Division of the work: all units' tiles in one line (beginning a unit counts UNIT_WEIGHT, a 16-bit tile TAIL_WEIGHT),

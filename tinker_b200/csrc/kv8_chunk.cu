@@ -662,6 +662,12 @@ int launch(Params& p, const Plan& pl, int head_dim, cudaStream_t st) {
 
 }  // namespace chunk
 
+// Sequences whose operands are laid out at once: the workspace stays below a gigabyte unless one alone needs more.
+static int sequences_at_once(int batch, int num_kv_heads, int64_t rows, int64_t len, int head_dim, int sm_count) {
+  const int64_t one = chunk::make_plan(1, num_kv_heads, rows, len, head_dim, sm_count).total;
+  return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(batch, (int64_t(1) << 30) / std::max<int64_t>(one, 1))));
+}
+
 bool chunk_fits(int batch, int num_heads, int num_kv_heads, int seq, int64_t len) {
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
   return rows >= CHUNK_MIN_ROWS && rows < (1 << 20) && len < (1 << 30) && batch <= 65535 &&
@@ -669,7 +675,11 @@ bool chunk_fits(int batch, int num_heads, int num_kv_heads, int seq, int64_t len
 }
 
 int64_t chunk_workspace(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int64_t len, int sm_count) {
-  return chunk::make_plan(batch, num_kv_heads, int64_t(num_heads / num_kv_heads) * seq, len, head_dim, sm_count).total;
+  // the largest over all lengths up to `len`: fewer sequences at once may need more than more of a shorter length
+  const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
+  const int n = sequences_at_once(batch, num_kv_heads, rows, len, head_dim, sm_count);
+  const int64_t here = chunk::make_plan(n, num_kv_heads, rows, len, head_dim, sm_count).total;
+  return n < batch ? std::max(here, int64_t(1) << 30) : here;
 }
 
 int chunk_attention(const Cache& c, const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs,
@@ -680,37 +690,48 @@ int chunk_attention(const Cache& c, const void* q, int64_t qs, const void* k, in
   Params p{};
   p.groups = num_heads / num_kv_heads;
   p.rows = p.groups * seq;
-  const Plan pl = make_plan(batch, num_kv_heads, p.rows, int64_t(start_pos) + seq, head_dim, sm_count);
-  p.q = q, p.qs = qs, p.k = k, p.ks = ks, p.v = v, p.vs = vs;
-  p.kc = static_cast<const uint8_t*>(c.k);
-  p.vc = static_cast<const uint8_t*>(c.v);
-  p.scales = c.scales;
-  p.tail = c.tail;
+  const int64_t len = int64_t(start_pos) + seq;
+  const int at_once = sequences_at_once(batch, num_kv_heads, p.rows, len, head_dim, sm_count);
+  p.qs = qs, p.ks = ks, p.vs = vs, p.os = os;
   p.num_blocks = c.num_blocks;
   p.cos_t = cos_t, p.sin_t = sin_t;
   p.start = start_pos;
   p.seq = seq;
   p.num_kv_heads = num_kv_heads;
-  p.batch = batch;
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
-  char* ws = static_cast<char*>(workspace);
-  p.qx = reinterpret_cast<__half*>(ws + pl.qx);
-  p.qf = reinterpret_cast<float*>(ws + pl.qf);
-  p.kx = reinterpret_cast<__half*>(ws + pl.kx);
-  p.vx = reinterpret_cast<__half*>(ws + pl.vx);
-  p.sx = reinterpret_cast<float4*>(ws + pl.sx);
-  p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
-  p.part_o = reinterpret_cast<float*>(ws + pl.o);
-  p.keys = static_cast<int>(pl.keys);
-  p.out = out;
-  p.os = os;
-  p.n_qtiles = pl.n_qtiles;
-  p.splits = pl.splits;
-  if (dtype == TK_F16)
-    return c.format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, pl, head_dim, st)
+  for (int b = 0; b < batch; b += at_once) {
+    p.batch = std::min(at_once, batch - b);
+    const Plan pl = make_plan(p.batch, num_kv_heads, p.rows, len, head_dim, sm_count);
+    const int64_t tok = int64_t(b) * seq, bh = int64_t(b) * num_kv_heads, block = int64_t(BLOCK) * head_dim;
+    p.q = static_cast<const char*>(q) + tok * qs * 2;
+    p.k = static_cast<const char*>(k) + tok * ks * 2;
+    p.v = static_cast<const char*>(v) + tok * vs * 2;
+    p.out = static_cast<char*>(out) + tok * os * 2;
+    p.kc = static_cast<const uint8_t*>(c.k) + bh * c.num_blocks * block;
+    p.vc = static_cast<const uint8_t*>(c.v) + bh * c.num_blocks * block;
+    p.scales = c.scales + bh * c.num_blocks * 2;
+    p.tail = static_cast<const char*>(c.tail) + bh * 2 * block * 2;
+    char* ws = static_cast<char*>(workspace);
+    p.qx = reinterpret_cast<__half*>(ws + pl.qx);
+    p.qf = reinterpret_cast<float*>(ws + pl.qf);
+    p.kx = reinterpret_cast<__half*>(ws + pl.kx);
+    p.vx = reinterpret_cast<__half*>(ws + pl.vx);
+    p.sx = reinterpret_cast<float4*>(ws + pl.sx);
+    p.part_ml = reinterpret_cast<float2*>(ws + pl.ml);
+    p.part_o = reinterpret_cast<float*>(ws + pl.o);
+    p.keys = static_cast<int>(pl.keys);
+    p.n_qtiles = pl.n_qtiles;
+    p.splits = pl.splits;
+    int rc;
+    if (dtype == TK_F16)
+      rc = c.format == TK_KV8_E4M3 ? launch<TK_F16, TK_KV8_E4M3>(p, pl, head_dim, st)
                                    : launch<TK_F16, TK_KV8_INT8>(p, pl, head_dim, st);
-  return c.format == TK_KV8_E4M3 ? launch<TK_BF16, TK_KV8_E4M3>(p, pl, head_dim, st)
-                                 : launch<TK_BF16, TK_KV8_INT8>(p, pl, head_dim, st);
+    else
+      rc = c.format == TK_KV8_E4M3 ? launch<TK_BF16, TK_KV8_E4M3>(p, pl, head_dim, st)
+                                   : launch<TK_BF16, TK_KV8_INT8>(p, pl, head_dim, st);
+    if (rc) return rc;
+  }
+  return TK_OK;
 }
 
 }  // namespace kv8

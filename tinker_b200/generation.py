@@ -158,7 +158,7 @@ class KVCache8:
         self.length = 0
         self.position = torch.zeros(1, dtype=torch.int32, device=device)
         self._layers = [KVCache8Layer(self, i) for i in range(num_layers)]
-        self._ws: dict = {}
+        self._ws: torch.Tensor | None = None
 
     @property
     def num_layers(self) -> int:
@@ -168,16 +168,15 @@ class KVCache8:
         return self._layers[i]
 
     def workspace(self, seq: int) -> torch.Tensor | None:
-        """Scratch for ``kv8_attention`` with ``seq`` new tokens at any position (shared by the layers, whose
-        kernels run one after another). One for each ``seq``: a captured step keeps the address of its own."""
-        need = kv8_attention_workspace(self.batch_size, self.num_heads, self.num_kv_heads, self.head_dim, seq,
-                                       self.capacity)
-        if need == 0:
+        """Scratch of a decode step (``seq`` 1) at any position, shared by the layers, whose kernels run one
+        after another; None for more tokens, whose operands the call lays out in memory of its own."""
+        if seq != 1:
             return None
-        ws = self._ws.get(seq)
-        if ws is None:
-            ws = self._ws[seq] = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
-        return ws
+        if self._ws is None:
+            need = kv8_attention_workspace(self.batch_size, self.num_heads, self.num_kv_heads, self.head_dim, 1,
+                                           self.capacity)
+            self._ws = torch.zeros(need, dtype=torch.uint8, device=self.k.device)
+        return self._ws
 
     def reset(self) -> None:
         self.length = 0

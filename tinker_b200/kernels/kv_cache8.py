@@ -158,12 +158,11 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
     out = q.new_empty((B, S, width))
     if B == 0 or S == 0:
         return out
-    if S == 1 or pos_ptr is not None:  # independent of the other sizes
-        need = _workspace_bytes(idx, 1, num_heads, num_kv_heads, head_dim, 1, 1)
-    else:
+    need = base = _workspace_bytes(idx, 1, num_heads, num_kv_heads, head_dim, 1, 1)  # independent of the other sizes
+    if S > 1 and pos_ptr is None:
         need = _workspace_bytes(idx, B, num_heads, num_kv_heads, head_dim, S, start_pos + S)
-    if workspace is None:
-        workspace = torch.zeros(need, dtype=torch.uint8, device=out.device)
+    if workspace is None:  # only the form for few rows counts on zeros
+        workspace = (torch.empty if need > base else torch.zeros)(need, dtype=torch.uint8, device=out.device)
     elif workspace.nbytes < need or workspace.get_device() != idx or not workspace.is_contiguous():
         raise ValueError(f"kv8_attention: workspace smaller than the {need} bytes needed, or not contiguous")
     launch(idx, "tk_kv8_attention", 1 if S == 1 else 2, _lib.lib().tk_kv8_attention, q.data_ptr(), qs, k.data_ptr(), ks,
