@@ -10,9 +10,9 @@ The score of a key carries the split's remainder (2^-22 |q k|) and D + 8 roundin
 error is that of the score on both sides of the quotient (twice, and twice for max - score), the exponential and the
 split of the weight add less than 2^-20, the fp32 sum over n keys at most n 2^-24.
 
-From 64 query rows of a kv head on, at a position known on the host, q and the weights are rounded to f16 once: 2^-12 of
-each of a score's terms (so 2^-12 S1 of a score, twice for the quotient) and 2^-12 of a weight. The bound then has
-2 max|v| (2^-11 S1 + 2^-12) more.
+From 64 query rows of a kv head on, at a position known on the host, the weights are rounded to f16 once, 2^-12 of a
+weight, and q where the result is bf16: 2^-12 of each of a score's terms, so 2^-12 S1 of a score, twice for the quotient.
+The bound then has 2 max|v| (2^-12 + 2^-11 S1 for bf16) more.
 """
 
 import math
@@ -92,7 +92,7 @@ def exact(q, k, v, cos, sin, rows, starts, hq, hkv, d, on_host=True):
             o = torch.softmax(s.masked_fill(future, -math.inf), -1) @ V
             out[b, :, h] = o
             tol[b, :, h] = torch.finfo(dtype).eps / 2 * o.abs() + 2 * V.abs().max() * (
-                4 * (d + 8) * 2.0 ** -24 * s1 + n * 2.0 ** -24 + 2.0 ** -20 + once * (2.0 ** -11 * s1 + 2.0 ** -12))
+                4 * (d + 8) * 2.0 ** -24 * s1 + n * 2.0 ** -24 + 2.0 ** -20 + once * (2.0 ** -12 + (dtype == torch.bfloat16) * 2.0 ** -11 * s1))
     return out.reshape(B, S, hq * d), tol.reshape(B, S, hq * d), k4.to(dtype), v4.to(dtype)
 
 

@@ -8,11 +8,11 @@
 //      k   [sequence, kv head, position, D], v [sequence, kv head, D, position]: codes as they are, rows of the open
 //          block and of the call times a power of two for each 32 tokens, zeros to the end of the last 128-key tile;
 //          with (scale_k, log2 scale_v, 1 / scale_v) of each 32 tokens beside them.
-//    Codes and scaled rows are exact in f16; q is rounded once, to 11 bits (the tensor cores take 16-bit operands, and
-//    a second product with the remainder would double their time): 2^-12 of a score's terms, as the rounding of the
-//    weights to f16 below is 2^-12 of a weight. Both lie under the rounding of a bf16 result by a factor of eight and
-//    are of the size of that of an fp16 result.
-// 2. kv8_chunk_kernel: a CTA takes two 128-row query tiles of one (sequence, kv head) - rows of all the heads that
+//    Codes and scaled rows are exact in f16; q is rounded to 11 bits, 2^-12 of each of a score's terms. Under a bf16
+//    result (2^-9) that does not show; for an fp16 result it would double the error (4.3e-4 instead of 2.1e-4 relative
+//    on 8-bit keys with strong channels), so there the remainder q - f16(q) is laid out too and has a product of its
+//    own. The weights are rounded to f16 once, 2^-12 of a weight, in both.
+// 2. kv8_chunk_kernel: a CTA takes two 128-row query tiles (fp16: one and its remainder) of one (sequence, kv head) - rows of all the heads that
 //    share it, so a key tile is loaded once for them - and a range of the 128-key tiles. One thread feeds a ring of K
 //    and V tiles by TMA, one issues S = Q K^T and O += P V as tcgen05.mma with S and O in tensor memory, two
 //    warpgroups (thread = query row) turn S into weights: x = s * (factor * scale_k) + log2 scale_v for each 32 keys, w =
@@ -74,7 +74,7 @@ struct Params {
   int start, seq, num_kv_heads, groups, rows, batch;
   float scale_log2;
   // what it writes
-  __half* qx;     // [batch, num_kv_heads, rows, D]
+  __half* qx;     // [batch, num_kv_heads, rows, D], then the remainders in the same layout
   float* qf;      // [batch, num_kv_heads, rows]
   __half* kx;     // [batch, num_kv_heads, keys, D]
   __half* vx;     // [batch, num_kv_heads, D, keys]
@@ -88,6 +88,9 @@ struct Params {
   float2* part_ml;  // [batch, num_kv_heads, rows, splits]
   float* part_o;    // [batch, num_kv_heads, rows, splits, D]
 };
+
+// fp16: a query tile's remainder takes the place of the second tile
+template <int DT> constexpr bool REMAINDER = DT == TK_F16;
 
 constexpr int EXPAND_WARPS = 8;  // 4 for keys, 4 for values
 
@@ -135,10 +138,21 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) kv8_expand_kernel(const Par
 #pragma unroll
     for (int o = 1; o < LANES; o <<= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
     const float up = to_f16_range(__float_as_uint(amax));
-    uint32_t y[8];
+    uint32_t y[8], z[8];
 #pragma unroll
-    for (int i = 0; i < 8; ++i) y[i] = h2_u32(__floats2half2_rn(f[2 * i] * up, f[2 * i + 1] * up));
+    for (int i = 0; i < 8; ++i) {
+      const __half2 hi = __floats2half2_rn(f[2 * i] * up, f[2 * i + 1] * up);
+      const float2 g = __half22float2(hi);
+      y[i] = h2_u32(hi);
+      z[i] = h2_u32(__floats2half2_rn(f[2 * i] * up - g.x, f[2 * i + 1] * up - g.y));
+    }
     if (valid) {
+      if constexpr (REMAINDER<DT>) {
+        const int64_t all = static_cast<int64_t>(p.batch) * p.num_kv_heads;
+        uint4* lo = reinterpret_cast<uint4*>(p.qx + ((all + bh) * p.rows + row) * D + part * 16);
+        lo[0] = make_uint4(z[0], z[1], z[2], z[3]);
+        lo[1] = make_uint4(z[4], z[5], z[6], z[7]);
+      }
       uint4* dst = reinterpret_cast<uint4*>(p.qx + (bh * p.rows + row) * D + part * 16);
       dst[0] = make_uint4(y[0], y[1], y[2], y[3]);
       dst[1] = make_uint4(y[4], y[5], y[6], y[7]);
@@ -263,15 +277,17 @@ __global__ void __launch_bounds__(THREADS, 1)
   uint64_t* bars = reinterpret_cast<uint64_t*>(smem + S::BAR_OFF);
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + S::NUM_BARS);
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int n_pairs = (p.n_qtiles + 1) >> 1;
+  constexpr bool LO = REMAINDER<DT>;
+  const int n_pairs = LO ? p.n_qtiles : (p.n_qtiles + 1) >> 1;
   const int pair = n_pairs - 1 - static_cast<int>(blockIdx.z) / p.splits;  // the longest first
   const int split = static_cast<int>(blockIdx.z) % p.splits;
   const int kvh = blockIdx.x, b = blockIdx.y;
   const int64_t bh = static_cast<int64_t>(b) * p.num_kv_heads + kvh;
   // key tiles that query tile x sees (0 if there is none), and this CTA's part of them
+  auto first_row = [&](int x) { return (LO ? pair : 2 * pair + x) * BQ; };
   auto tiles_of = [&](int x) {
-    const int first = (2 * pair + x) * BQ;
-    if (first >= p.rows) return 0;
+    const int first = first_row(x);
+    if (first >= p.rows || (LO && x == 1)) return 0;
     return (p.start + (min(p.rows, first + BQ) - 1) / p.groups) / BKV + 1;
   };
   const int all_a = tiles_of(0), all_b = tiles_of(1), all = max(all_a, all_b);
@@ -310,12 +326,14 @@ __global__ void __launch_bounds__(THREADS, 1)
       prefetch_tmap(&tk);
       prefetch_tmap(&tv);
       pdl_wait();  // the operands are written by the expansion
-      const int n_q = n_kv == 0 ? 0 : all_b > 0 ? 2 : 1, bhi = static_cast<int>(bh);  // no copy that nobody waits for
+      const int n_q = n_kv == 0 ? 0 : LO || all_b > 0 ? 2 : 1;  // no copy that nobody waits for
+      const int bhi = static_cast<int>(bh), all_bh = p.batch * p.num_kv_heads;
       if (n_q > 0) mbar_arrive_expect_tx(bars + B_Q_FULL, n_q * S::Q_BYTES);
       for (int t = 0; t < n_q; ++t)
 #pragma unroll
         for (int cb = 0; cb < D / 64; ++cb)
-          tma_load_3d(smem + t * S::Q_BYTES + cb * 128 * 128, &tq, bars + B_Q_FULL, cb * 64, (2 * pair + t) * BQ, bhi);
+          tma_load_3d(smem + t * S::Q_BYTES + cb * 128 * 128, &tq, bars + B_Q_FULL, cb * 64, first_row(t),
+                      bhi + (LO ? t * all_bh : 0));
       for (int i = 0; i < 2 * n_kv; ++i) {
         const int slot = i % NS;
         if (i >= NS && !mbar_wait(bars + B_EMPTY + slot, ((i / NS) - 1) & 1)) break;
@@ -339,10 +357,13 @@ __global__ void __launch_bounds__(THREADS, 1)
       constexpr uint32_t idesc_o = make_idesc_f16(Dt<TK_F16>::umma_fmt, BQ, D, 0, 0);
       auto issue_s = [&](uint64_t q_desc, uint64_t k_desc, uint32_t t_s) {
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint64_t off16 = static_cast<uint64_t>(((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4);
-          umma_f16_ss(t_s, q_desc + off16, k_desc + off16, idesc_s, kk != 0);
-        }
+        for (int lo = 0; lo <= (LO ? 1 : 0); ++lo)
+#pragma unroll
+          for (int kk = 0; kk < D / 16; ++kk) {
+            const uint64_t off16 = static_cast<uint64_t>(((kk >> 2) * (128 * 128) + (kk & 3) * 32) >> 4);
+            umma_f16_ss(t_s, q_desc + static_cast<uint64_t>(lo * S::Q_BYTES / 16) + off16, k_desc + off16, idesc_s,
+                        lo + kk != 0);
+          }
       };
       auto issue_pv = [&](uint64_t p_desc, uint64_t v_desc, uint32_t t_o, bool acc) {
 #pragma unroll
@@ -409,7 +430,7 @@ __global__ void __launch_bounds__(THREADS, 1)
     }
   } else if (warp < SOFTMAX_WARPS) {
     const int x = warp >> 2, r = tid & 127;
-    const int row = (2 * pair + x) * BQ + r;
+    const int row = first_row(x) + r;
     const int n_x = x == 0 ? n_a : n_b;
     const uint32_t lane_off = static_cast<uint32_t>((warp & 3) * 32) << 16;
     const uint32_t t_s = tmem_base + x * 128, t_o = tmem_base + 256 + x * D;
@@ -421,7 +442,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool valid = row < p.rows;
       const float cq = valid ? __ldcg(p.qf + bh * p.rows + row) : 0.f;
       const int qpos = p.start + (valid ? row : p.rows - 1) / p.groups;
-      const int first_pos = p.start + (2 * pair + x) * BQ / p.groups;  // of the tile's first row: keys to there are open
+      const int first_pos = p.start + first_row(x) / p.groups;  // of the tile's first row: keys to there are open
       const float4* sx = p.sx + bh * (p.keys / BLOCK) + static_cast<int64_t>(lo) * (BKV / BLOCK);
       for (int j = 0; ok && j < n_x; ++j) {
         float4 sc[4];  // from L1: one line holds two tiles' and the line after it is on its way
@@ -595,11 +616,11 @@ struct Plan {
 };
 
 // Splits of the key axis: as many as CTAs fit on the GPU at once, with four key tiles or more each.
-Plan make_plan(int batch, int num_kv_heads, int64_t rows, int64_t len, int head_dim, int sm_count) {
+Plan make_plan(int batch, int num_kv_heads, int64_t rows, int64_t len, int head_dim, bool remainder, int sm_count) {
   Plan pl{};
   pl.n_qtiles = static_cast<int>((rows + BQ - 1) / BQ);
   pl.keys = (len + BKV - 1) / BKV * BKV;
-  const int64_t units = int64_t(batch) * num_kv_heads * ((pl.n_qtiles + 1) / 2);
+  const int64_t units = int64_t(batch) * num_kv_heads * (remainder ? pl.n_qtiles : (pl.n_qtiles + 1) / 2);
   pl.splits = static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(sm_count / units, pl.keys / BKV / 4)));
   const int64_t bh = int64_t(batch) * num_kv_heads;
   int64_t at = 0;
@@ -608,7 +629,7 @@ Plan make_plan(int batch, int num_kv_heads, int64_t rows, int64_t len, int head_
     at += up256(bytes);
     return x;
   };
-  pl.qx = take(bh * rows * head_dim * 2);
+  pl.qx = take(bh * rows * head_dim * (remainder ? 4 : 2));
   pl.qf = take(bh * rows * 4);
   pl.kx = take(bh * pl.keys * head_dim * 2);
   pl.vx = take(bh * pl.keys * head_dim * 2);
@@ -623,7 +644,7 @@ template <int DT, int FMT, int D>
 int launch(Params& p, const Plan& pl, cudaStream_t st) {
   const uint64_t bh = uint64_t(p.batch) * p.num_kv_heads;
   CUtensorMap tq, tk_, tv;
-  if (int rc = tensor_map_3d(&tq, p.qx, TK_F16, D, p.rows, bh, D, uint64_t(p.rows) * D, 64, BQ, 1)) return rc;
+  if (int rc = tensor_map_3d(&tq, p.qx, TK_F16, D, p.rows, REMAINDER<DT> ? 2 * bh : bh, D, uint64_t(p.rows) * D, 64, BQ, 1)) return rc;
   if (int rc = tensor_map_3d(&tk_, p.kx, TK_F16, D, p.keys, bh, D, uint64_t(p.keys) * D, 64, BKV, 1)) return rc;
   if (int rc = tensor_map_3d(&tv, p.vx, TK_F16, p.keys, D, bh, p.keys, uint64_t(p.keys) * D, 64, D, 1)) return rc;
   auto kern = kv8_chunk_kernel<DT, D>;
@@ -647,7 +668,7 @@ int launch(Params& p, const Plan& pl, cudaStream_t st) {
   if (int rc = launch_kernel(expand, dim3(p.q_ctas + k_ctas, p.num_kv_heads, p.batch), dim3(EXPAND_WARPS * 32),
                              EXPAND_SMEM, st, 1, "kv8_expand", p))
     return rc;
-  if (int rc = launch_kernel(kern, dim3(p.num_kv_heads, p.batch, (p.n_qtiles + 1) / 2 * p.splits), dim3(THREADS),
+  if (int rc = launch_kernel(kern, dim3(p.num_kv_heads, p.batch, (REMAINDER<DT> ? p.n_qtiles : (p.n_qtiles + 1) / 2) * p.splits), dim3(THREADS),
                              Smem<D>::TOTAL, st, 1, "kv8_chunk", tq, tk_, tv, p))
     return rc;
   if (p.splits == 1) return TK_OK;
@@ -662,9 +683,15 @@ int launch(Params& p, const Plan& pl, int head_dim, cudaStream_t st) {
 
 }  // namespace chunk
 
+// Workspace of a plan, whichever the type.
+static int64_t chunk_total(int batch, int num_kv_heads, int64_t rows, int64_t len, int head_dim, int sm_count) {
+  return std::max(chunk::make_plan(batch, num_kv_heads, rows, len, head_dim, true, sm_count).total,
+                  chunk::make_plan(batch, num_kv_heads, rows, len, head_dim, false, sm_count).total);
+}
+
 // Sequences whose operands are laid out at once: the workspace stays below a gigabyte unless one alone needs more.
 static int sequences_at_once(int batch, int num_kv_heads, int64_t rows, int64_t len, int head_dim, int sm_count) {
-  const int64_t one = chunk::make_plan(1, num_kv_heads, rows, len, head_dim, sm_count).total;
+  const int64_t one = chunk_total(1, num_kv_heads, rows, len, head_dim, sm_count);
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(batch, (int64_t(1) << 30) / std::max<int64_t>(one, 1))));
 }
 
@@ -678,7 +705,7 @@ int64_t chunk_workspace(int batch, int num_heads, int num_kv_heads, int head_dim
   // the largest over all lengths up to `len`: fewer sequences at once may need more than more of a shorter length
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
   const int n = sequences_at_once(batch, num_kv_heads, rows, len, head_dim, sm_count);
-  const int64_t here = chunk::make_plan(n, num_kv_heads, rows, len, head_dim, sm_count).total;
+  const int64_t here = chunk_total(n, num_kv_heads, rows, len, head_dim, sm_count);
   return n < batch ? std::max(here, int64_t(1) << 30) : here;
 }
 
@@ -701,7 +728,7 @@ int chunk_attention(const Cache& c, const void* q, int64_t qs, const void* k, in
   p.scale_log2 = static_cast<float>((1.0 / std::sqrt(double(head_dim))) * 1.4426950408889634);
   for (int b = 0; b < batch; b += at_once) {
     p.batch = std::min(at_once, batch - b);
-    const Plan pl = make_plan(p.batch, num_kv_heads, p.rows, len, head_dim, sm_count);
+    const Plan pl = make_plan(p.batch, num_kv_heads, p.rows, len, head_dim, dtype == TK_F16, sm_count);
     const int64_t tok = int64_t(b) * seq, bh = int64_t(b) * num_kv_heads, block = int64_t(BLOCK) * head_dim;
     p.q = static_cast<const char*>(q) + tok * qs * 2;
     p.k = static_cast<const char*>(k) + tok * ks * 2;
