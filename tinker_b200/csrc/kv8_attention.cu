@@ -16,9 +16,13 @@
 //     w = 2^(x + log2 scale_v - m), m the running maximum of that sum, O = sum w * code, and the softmax's
 //     denominator is sum w / scale_v. So O needs no pass per block, w stays in [0, 1], and the rounding of log2
 //     scale_v cancels between numerator and denominator.
-// (The keys as columns, with f16(q) and remainder as two halves of the 16 rows, took 274 instead of some 170
-// instructions for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 18.8 us for 64
-// sequences of 4 kv heads at 2047.)
+// (The keys as columns, with f16(q) and remainder as two halves of the 16 rows, took 274 instead of 231 instructions
+// for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 18.7 us for 64 sequences of 4
+// kv heads at 2047.)
+//
+// Bound by HBM at D = 128 (16 x 16001 positions of 8 kv heads: 87 us, 6.0 TB/s), at D = 64 by the instructions of a tile
+// as much (48 ragged sequences of 8 kv heads: 45.6 us, 4.5 TB/s; int8 costs 97 instructions more than e4m3), for
+// little work by the chain position - copies - products - merge (7 us for one sequence of 4 kv heads at 127).
 //
 // Division of the work: all units' tiles in one line (beginning a unit counts UNIT_WEIGHT, a 16-bit tile TAIL_WEIGHT),
 // cut into equal pieces, one for each warp that fits on the GPU at once. So long and short sequences, few units and
