@@ -537,3 +537,29 @@ def test_chunk_of_more_sequences_than_are_laid_out_at_once():
     for b in (0, 7, 12, 13, 15):
         want, tol, _, _ = exact(q[b:b + 1], k[b:b + 1], v[b:b + 1], None, None, rows[b:b + 1], [n], hq, hkv, d)
         assert ((out[b:b + 1].double() - want).abs() <= tol).all(), b
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [9, 40])  # 18 and 80 query rows of a kv head: the one form and the other
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+def test_tokens_that_are_not_finite_stay_behind_the_mask(S, dt, what, bad):
+    """A NaN or an infinity in a later token of a chunk: the rows before it are what they are without it, in both forms;
+    the rows that see a value that is not finite are NaN."""
+    require_b200()
+    from tinker_b200.kernels import kv8_attention
+    dtype, hq, hkv, d, n, at = DTYPES[dt], 8, 4, 64, 130, 6
+    g = torch.Generator(device="cuda").manual_seed(S)
+    kc, vc, sc, tail, rows = make_cache(2, hkv, d, 256, [n, n], dtype, "e4m3", g, garbage=False)
+    w = torch.randn(2, S, (hq + 2 * hkv) * d, device="cuda", generator=g).to(dtype)
+    q, k, v = (t.contiguous() for t in w.split([hq * d, hkv * d, hkv * d], -1))
+    want, tol, _, _ = exact(q, k, v, None, None, rows, [n, n], hq, hkv, d)
+    (k if what == "k" else v)[0, at, d + 3] = bad  # sequence 0, kv head 1: heads 2 and 3
+    out = kv8_attention(q, k, v, None, None, kc, vc, sc, tail, hq, hkv, d, start_pos=n).double()
+    ok = torch.ones(2, S, hq * d, dtype=torch.bool, device="cuda")
+    ok[0, at:, 2 * d:4 * d] = False
+    assert torch.isfinite(out[ok]).all()
+    assert ((out - want).abs() <= tol)[ok].all()
+    if what == "v":
+        assert torch.isnan(out[0, at:, 2 * d:4 * d]).all()

@@ -120,6 +120,13 @@ __device__ __forceinline__ uint32_t amax2_warp(uint32_t m) {
   return max(m & 0xffffu, m >> 16);
 }
 
+// Whether a 16-byte chunk holds a NaN or an infinity.
+template <int DT>
+__device__ __forceinline__ bool not_finite(uint4 x) {
+  const uint32_t m = amax2(amax2(amax2(amax2(0u, x.x), x.y), x.z), x.w);
+  return max(m & 0xffffu, m >> 16) >= (DT == TK_F16 ? 0x7c00u : 0x7f80u);
+}
+
 // A warp's 16-bit tile in shared memory: 32 rows of D elements in 16-byte chunks, chunk c of row t at c ^ swz(t),
 // which keeps both the column fragments (rows 8a + e) and the row fragments free of bank conflicts.
 __device__ __forceinline__ int swz(int t) { return (t & 1) | (((t >> 3) & 3) << 1); }

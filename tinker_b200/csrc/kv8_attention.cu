@@ -586,6 +586,26 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
       }
       __syncwarp();
       uint32_t km = 0, vm = 0;
+      if (p.seq > 1) {
+        // Values that are not finite must not reach the rows that do not see their token (0 * NaN): the token's key
+        // becomes NaN, which the mask hides from those rows and which makes the others NaN, and its values 0.
+        uint32_t bad = 0;
+#pragma unroll 1
+        for (int idx = lane; idx < BLOCK * C16; idx += 32)
+          if (not_finite<DT>(*reinterpret_cast<const uint4*>(vtile + tile_off<D>(idx / C16, idx % C16))))
+            bad |= 1u << (idx / C16);
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        if (bad) {
+#pragma unroll 1
+          for (int idx = lane; idx < BLOCK * C16; idx += 32) {
+            if (!(bad >> (idx / C16) & 1)) continue;
+            const uint32_t off = tile_off<D>(idx / C16, idx % C16);
+            *reinterpret_cast<uint4*>(ktile + off) = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            *reinterpret_cast<uint4*>(vtile + off) = make_uint4(0, 0, 0, 0);
+          }
+          __syncwarp();
+        }
+      }
       if (DT == TK_BF16 || open + p.seq == BLOCK) {
 #pragma unroll 4
         for (int i = 0; i < C16; ++i) {  // any order of the tile's chunks

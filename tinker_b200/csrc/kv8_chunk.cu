@@ -20,8 +20,8 @@
 //    2^8. The scales cost nothing per score: the FMA of the softmax takes them as its factor and addend.
 // 3. With the key axis split (few query tiles), kv8_join_kernel merges the parts in their order.
 // Bound by the softmax's latency: products and exponentials take some 2000 cycles each for a pair of tiles at D = 128, a
-// step some 6000 (8 softmax warps on 4 schedulers). 512 tokens of 32 heads of 128 at 7001: 123 us in all, 95 of them
-// here (128 CTAs), the rest the expansion, the join and the append; 154 us for fp16. kv8_attention.cu took 641 us.
+// step some 6000 (8 softmax warps on 4 schedulers). 512 tokens of 32 heads of 128 at 7001: 129 us in all, 100 of them
+// here (128 CTAs), the rest the expansion, the join and the append; 160 us for fp16. kv8_attention.cu took 641 us.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -80,7 +80,7 @@ struct Params {
   float* qf;      // [batch, num_kv_heads, rows]
   __half* kx;     // [batch, num_kv_heads, keys, D]
   __half* vx;     // [batch, num_kv_heads, D, keys]
-  float4* sx;     // [batch, num_kv_heads, keys / 32]: scale_k, log2 scale_v, 1 / scale_v
+  float4* sx;     // [batch, num_kv_heads, keys / 32]: scale_k, log2 scale_v, 1 / scale_v, tokens to be NaN (bits)
   int keys;       // start + seq, rounded up to whole key tiles
   int q_ctas;     // expansion CTAs that lay out q
   // the attention
@@ -97,7 +97,7 @@ template <int DT> constexpr bool REMAINDER = DT == TK_F16;
 constexpr int EXPAND_WARPS = 8;  // 4 for keys, 4 for values
 
 template <int DT, int FMT, int D>
-__global__ void __launch_bounds__(EXPAND_WARPS * 32) kv8_expand_kernel(const Params p) {
+__global__ void __launch_bounds__(EXPAND_WARPS * 32, 2) kv8_expand_kernel(const Params p) {
   extern __shared__ __align__(128) uint8_t smem[];
   using T = typename Dt<DT>::T;
   constexpr int C16 = D / 8;
@@ -217,7 +217,7 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) kv8_expand_kernel(const Par
   const int64_t stride = values ? p.vs : p.ks;
   const int row0 = (block - n8) * BLOCK - open;  // the call's row of the block's first token
   uint8_t* tile = smem + warp * (BLOCK * D * 2);
-  uint32_t m = 0;
+  uint32_t m = 0, bad = 0;
   uint4 x[C16];
 #pragma unroll
   for (int i = 0; i < C16; ++i) {  // all loads in flight, then the rotations
@@ -232,6 +232,15 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) kv8_expand_kernel(const Par
       const int64_t ang = (static_cast<int64_t>(p.start) + s) * (D / 2) + c * 4;
       rope_chunk<DT>(x[i], p.cos_t + ang, p.sin_t + ang);
     }
+    if (values && not_finite<DT>(x[i])) bad |= 1u << t;
+  }
+  // A token whose values are not finite must not reach the rows that do not see it (0 * NaN): its values become 0, and
+  // the rows that see it NaN by its scores.
+  bad = __reduce_or_sync(0xffffffffu, bad);
+#pragma unroll
+  for (int i = 0; i < C16; ++i) {
+    const int idx = lane + 32 * i, t = idx / C16, c = idx % C16;
+    if (bad >> t & 1) x[i] = make_uint4(0, 0, 0, 0);
     m = amax2(amax2(amax2(amax2(m, x[i].x), x[i].y), x[i].z), x[i].w);
     *reinterpret_cast<uint4*>(tile + tile_off<D>(t, c)) = x[i];
   }
@@ -262,7 +271,7 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32) kv8_expand_kernel(const Par
       *reinterpret_cast<uint4*>(vx + static_cast<int64_t>(8 * n + r) * p.keys + 8 * q) =
           make_uint4(to_half(x[0]), to_half(x[1]), to_half(x[2]), to_half(x[3]));
     }
-    if (lane == 0) sx[1] = -__log2f(up), sx[2] = up;
+    if (lane == 0) sx[1] = -__log2f(up), sx[2] = up, sx[3] = __uint_as_float(bad);
   }
 }
 
@@ -444,7 +453,7 @@ __global__ void __launch_bounds__(THREADS, 1)
       const bool valid = row < p.rows;
       const float cq = valid ? __ldcg(p.qf + bh * p.rows + row) : 0.f;
       const int qpos = p.start + (valid ? row : p.rows - 1) / p.groups;
-      const int first_pos = p.start + first_row(x) / p.groups;  // of the tile's first row: keys to there are open
+      const int rows16 = p.start / BLOCK * BLOCK;  // the first position that is kept in 16 bits; no row's own is below it
       const float4* sx = p.sx + bh * (p.keys / BLOCK) + static_cast<int64_t>(lo) * (BKV / BLOCK);
       for (int j = 0; ok && j < n_x; ++j) {
         float4 sc[4];  // from L1: one line holds two tiles' and the line after it is on its way
@@ -458,10 +467,12 @@ __global__ void __launch_bounds__(THREADS, 1)
         tc_fence_before();
         mbar_arrive(bars + B_S_FREE + x);
         const int key = (lo + j) * BKV;
-        if (key + BKV - 1 > first_pos) {
+        if (key + BKV > rows16) {  // the open block and the call's own tokens: the mask, and tokens that are NaN
 #pragma unroll
-          for (int c = 0; c < BKV; ++c)
+          for (int c = 0; c < BKV; ++c) {
+            if (__float_as_uint(sc[c >> 5].w) >> (c & 31) & 1) sv[c] = __uint_as_float(0x7fc00000u);
             if (key + c > qpos) sv[c] = -INFINITY;
+          }
         }
         // the maximum of x: for each 32 keys that of the raw products, times their factor
         float f[4], mx = -INFINITY;
