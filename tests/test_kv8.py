@@ -563,3 +563,59 @@ def test_tokens_that_are_not_finite_stay_behind_the_mask(S, dt, what, bad):
     assert ((out - want).abs() <= tol)[ok].all()
     if what == "v":
         assert torch.isnan(out[0, at:, 2 * d:4 * d]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("who, gap", [("own", 10.0), ("own", 14.0), ("first", 13.0)])
+@pytest.mark.parametrize("S", [1, 9, 40])  # 40: 80 query rows of a kv head, the tensor-core form
+@pytest.mark.parametrize("size", [0.05, 0.002])
+@pytest.mark.parametrize("dt, code", [("fp16", "e4m3"), ("fp16", "int8"), ("bf16", "e4m3")])
+def test_small_weights_beside_a_dominant_token(dt, code, size, S, who, gap):
+    """One token's score lies far above thousands of others that make up a part of the result together: the weights of
+    those keep their bits, whatever the values' scales. `own`: the query's own token, in 16 bits; `first`: the first one,
+    whose block has a hundred times the others' scale. Values have a mean, so weights that the sum of values loses and the
+    denominator keeps would show.
+
+    A relative error e of the weights moves o by at most 2 e sum p |v|; e is that of the module's head. To it comes half of
+    f16's smallest number, 2^-25, where the largest weight f is 2^11 (tensor cores) or 2^15: with a weight w and a code c
+    for each key o is sum w c / (w_f / scale_f), c = v / scale, so it moves by at most 2^-36 (2^-40) r sum |v|, r the scale
+    of the dominant token's block over the least (1 for `own`, whose tile has the smaller one; 200 for `first`)."""
+    require_b200()
+    from tinker_b200.kernels import kv8_append, kv8_attention, kv8_dequantize, kv8_empty
+    dtype, B, hq, hkv, d, n = DTYPES[dt], 20, 16, 8, 128, 7000
+    g = torch.Generator(device="cuda").manual_seed(S)
+    cache = kv8_empty(B, hkv, d, n + S, dtype, CODES[code])
+    q = torch.randn(B, S, hq // hkv, hkv, d, device="cuda", generator=g)
+    q[:, :, 1:] = q[:, :, :1] * (1 + 0.05 * torch.randn(B, S, hq // hkv - 1, hkv, 1, device="cuda", generator=g))
+    q = q.transpose(2, 3)  # the heads of a kv head look the same way
+    if who == "first":
+        q[:] = q[:, :1]
+    kn = q[:, :, :, 0] * (gap * math.sqrt(d) / q[:, :, :, 0].square().sum(-1, keepdim=True))
+    k = torch.randn(B, n, hkv, d, device="cuda", generator=g) * 0.02
+    v = size * (1 + 0.3 * torch.randn(B, n, hkv, d, device="cuda", generator=g))
+    vn = size * (1 + 0.3 * torch.randn(B, S, hkv, d, device="cuda", generator=g))
+    if who == "first":
+        k[:, 0], kn = kn[:, 0], torch.randn(B, S, hkv, d, device="cuda", generator=g) * 0.02
+        k[:, 1:32] = 0
+        v[:, 1] *= 100
+    q, kn, vn, k, v = (t.reshape(B, t.shape[1], -1).to(dtype) for t in (q, kn, vn, k, v))
+    kv8_append(k, v, *cache, 0)
+    rows = {b: torch.cat([t.double() for t in kv8_dequantize(*(t[b:b + 1] for t in cache), n)]) for b in (0, B - 1)}
+    out = kv8_attention(q, kn, vn, None, None, *cache, hq, hkv, d, start_pos=n).double().reshape(B, S, hq, d)
+    once = hq // hkv * S >= 64
+    for b in rows:
+        for h in range(hq):
+            x, j = q[b, :, h * d:(h + 1) * d].double(), h // (hq // hkv)
+            K = torch.cat([rows[b][0, j], kn[b, :, j * d:(j + 1) * d].double()])
+            V = torch.cat([rows[b][1, j], vn[b, :, j * d:(j + 1) * d].double()])
+            s = x @ K.T / math.sqrt(d)
+            s1 = (x.abs() @ K.abs().T / math.sqrt(d)).max()
+            future = torch.arange(n + S, device="cuda")[None] > n + torch.arange(S, device="cuda")[:, None]
+            p = torch.softmax(s.masked_fill(future, -math.inf), -1)
+            e = 4 * (d + 8) * 2.0 ** -24 * s1 + n * 2.0 ** -24 + 2.0 ** -20
+            e += once * (2.0 ** -12 + (dtype == torch.bfloat16) * 2.0 ** -11 * s1)
+            tol = torch.finfo(dtype).eps / 2 * (p @ V).abs() + 2 * e * (p @ V.abs())
+            tol += torch.finfo(dtype).tiny * torch.finfo(dtype).eps / 2  # half a step of a result below the normal numbers
+            tol += (2.0 ** -36 if once else 2.0 ** -40) * (200 if who == "first" else 1) * V.abs().sum(0)
+            err = (out[b, :, h] - p @ V).abs()
+            assert (err <= tol).all(), f"error / bound {(err / tol).max().item()}"

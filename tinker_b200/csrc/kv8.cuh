@@ -95,6 +95,21 @@ __device__ __forceinline__ float to_f16_range(uint32_t amax_bits) {
   return __uint_as_float(static_cast<uint32_t>(min(187, 268 - e)) << 23);
 }
 
+// The power of two that 16-bit values are multiplied by before they are operands in f16; from the 16-bit pattern of their
+// largest magnitude. It belongs to the weights' exponent as a block's scale does, so it has to bring the tile near the
+// codes' magnitudes: with f16 values of 0.05 taken as they are, a dominant token of this tile left the weights of encoded
+// blocks 2^-13 lower than its own, below what f16 holds. f16 goes up only, which is exact, and by 2^15 at most, so that one
+// packed product does it.
+template <int DT>
+__device__ __forceinline__ float value_factor(uint32_t amax_bits) {
+  if constexpr (DT == TK_F16) {
+    const float a = __half2float(__ushort_as_half(static_cast<unsigned short>(amax_bits)));
+    return fminf(fmaxf(to_f16_range(__float_as_uint(a)), 1.f), 32768.f);
+  } else {
+    return to_f16_range(amax_bits << 16);
+  }
+}
+
 template <int DT>
 __device__ __forceinline__ float2 unpack2(uint32_t w) {
   return Dt<DT>::unpack(*reinterpret_cast<const typename Dt<DT>::T2*>(&w));

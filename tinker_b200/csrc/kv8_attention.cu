@@ -8,14 +8,15 @@
 // Products: m16n8k16 with f16 operands and fp32 sums, a warp for each tile of 32 keys, with the keys (and the columns
 // of V) as the 16 rows of the product and the query rows as its 8 columns:
 //   * codes are exact in f16, so are 16-bit rows times a power of two that brings the tile's largest magnitude to
-//     [2^14, 2^15) (bf16; its 8 bits stay whole for 28 binades below that);
+//     [2^14, 2^15) (bf16; its 8 bits stay whole for 28 binades below that; f16 keys are taken as they are);
 //   * a query row takes two columns, f16(q) and the remainder q - f16(q), likewise its probabilities, whose sum stays
-//     in one lane: nothing is lost to 16-bit operands. Four query rows fill the 8 columns, which is what GQA with up
-//     to four heads for each kv head needs; eight rows (NG = 2) take every product twice;
+//     in one lane: 22 bits of each. Four query rows fill the 8 columns, which is what GQA with up to four heads for each
+//     kv head needs; eight rows (NG = 2) take every product twice;
 //   * the scale of a block's values goes into the exponent: with x = s * scale_k / sqrt(D) * log2 e, a weight is
-//     w = 2^(x + log2 scale_v - m), m the running maximum of that sum, O = sum w * code, and the softmax's
-//     denominator is sum w / scale_v. So O needs no pass per block, w stays in [0, 1], and the rounding of log2
-//     scale_v cancels between numerator and denominator.
+//     w = 2^(x + log2 scale_v - m + HEADROOM), m the running maximum of x + log2 scale_v, O = sum w * code, and the
+//     softmax's denominator is sum w / scale_v. So O needs no pass per block, and the rounding of log2 scale_v cancels
+//     between numerator and denominator. w goes up to 2^15, the top of f16's range, so that a weight is lost to its
+//     smallest number, 2^-24, only 2^40 below the largest: a million of them are still 2^-20 of the result.
 // (The keys as columns, with f16(q) and remainder as two halves of the 16 rows, took 274 instead of 231 instructions
 // for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 18.7 us for 64 sequences of 4
 // kv heads at 2047.)
@@ -54,6 +55,7 @@ constexpr int UNIT_WEIGHT = 1;  // and beginning a unit
 constexpr int PIECE_MIN = 4;    // weight of a piece when there is little work
 constexpr int MERGE_COST = 8;   // weight that a warp could take while the parts of two CTAs are merged
 constexpr int GROUP = 16;       // CTAs that are merged in one step
+constexpr float HEADROOM = 15.f;  // log2 of the largest weight
 
 struct AttnParams {
   const void* q;
@@ -197,7 +199,7 @@ __device__ __forceinline__ void attend_tiles(Rows<D, NG>& st, const uint32_t (&q
     uint32_t pf[NG][4];
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
-      const float base = mn[g] == -INFINITY ? 0.f : mn[g];  // a row that has seen no key yet: all weights 0
+      const float base = mn[g] == -INFINITY ? 0.f : mn[g] - HEADROOM;  // a row that has seen no key yet: all weights 0
       float sum = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
@@ -606,23 +608,20 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
           __syncwarp();
         }
       }
-      if (DT == TK_BF16 || open + p.seq == BLOCK) {
 #pragma unroll 4
-        for (int i = 0; i < C16; ++i) {  // any order of the tile's chunks
-          const uint4 kx = *reinterpret_cast<const uint4*>(ktile + (lane + 32 * i) * 16);
-          const uint4 vx = *reinterpret_cast<const uint4*>(vtile + (lane + 32 * i) * 16);
-          km = amax2(amax2(amax2(amax2(km, kx.x), kx.y), kx.z), kx.w);
-          vm = amax2(amax2(amax2(amax2(vm, vx.x), vx.y), vx.z), vx.w);
-        }
-        km = amax2_warp(km);
-        vm = amax2_warp(vm);
+      for (int i = 0; i < C16; ++i) {  // any order of the tile's chunks
+        const uint4 kx = *reinterpret_cast<const uint4*>(ktile + (lane + 32 * i) * 16);
+        const uint4 vx = *reinterpret_cast<const uint4*>(vtile + (lane + 32 * i) * 16);
+        km = amax2(amax2(amax2(amax2(km, kx.x), kx.y), kx.z), kx.w);
+        vm = amax2(amax2(amax2(amax2(vm, vx.x), vx.y), vx.z), vx.w);
       }
+      km = amax2_warp(km);
+      vm = amax2_warp(vm);
 
-      // f16 takes its own rows as they are; bf16 rows are brought to its range
-      const float fk = DT == TK_F16 ? 1.f : to_f16_range(km << 16), fv = DT == TK_F16 ? 1.f : to_f16_range(vm << 16);
+      const float fk = DT == TK_F16 ? 1.f : to_f16_range(km << 16), fv = value_factor<DT>(vm);
       auto to_half = [](uint32_t w, float f) -> uint32_t {
         if constexpr (DT == TK_F16) {
-          return w;
+          return h2_u32(__hmul2(u32_h2(w), __float2half2_rn(f)));
         } else {
           const float2 v = unpack2<DT>(w);
           return h2_u32(__floats2half2_rn(v.x * f, v.y * f));
@@ -639,10 +638,10 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
 #pragma unroll
             for (int e = 0; e < 2; ++e) {
               const uint4 x = *reinterpret_cast<const uint4*>(ktile + tile_off<D>(row, 8 * h + 2 * q + e));
-              w[4 * e] = to_half(x.x, fk);
-              w[4 * e + 1] = to_half(x.y, fk);
-              w[4 * e + 2] = to_half(x.z, fk);
-              w[4 * e + 3] = to_half(x.w, fk);
+              w[4 * e] = DT == TK_F16 ? x.x : to_half(x.x, fk);
+              w[4 * e + 1] = DT == TK_F16 ? x.y : to_half(x.y, fk);
+              w[4 * e + 2] = DT == TK_F16 ? x.z : to_half(x.z, fk);
+              w[4 * e + 3] = DT == TK_F16 ? x.w : to_half(x.w, fk);
             }
           },
           [&](int, int m, uint32_t (&w)[8]) {

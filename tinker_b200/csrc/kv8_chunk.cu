@@ -6,18 +6,19 @@
 //      q   [sequence, kv head, token * groups + head, D], rotated in fp32, times a power of two that brings the row to
 //          [2^14, 2^15), with the row's factor (scale log2 e / that power) beside it
 //      k   [sequence, kv head, position, D], v [sequence, kv head, D, position]: codes as they are, rows of the open
-//          block and of the call times a power of two for each 32 tokens, zeros to the end of the last 128-key tile;
-//          with (scale_k, log2 scale_v, 1 / scale_v) of each 32 tokens beside them.
+//          block and of the call times a power of two for each 32 tokens (f16 keys as they are), zeros to the end of the
+//          last 128-key tile; with (scale_k, log2 scale_v, 1 / scale_v) of each 32 tokens beside them.
 //    Codes and scaled rows are exact in f16; q is rounded to 11 bits, 2^-12 of each of a score's terms. Under a bf16
 //    result (2^-9) that does not show; for an fp16 result it would double the error (4.3e-4 instead of 2.1e-4 relative
 //    on 8-bit keys with strong channels), so there the remainder q - f16(q) is laid out too and has a product of its
-//    own. The weights are rounded to f16 once, 2^-12 of a weight, in both.
+//    own. The weights are rounded to f16 once, 2^-12 of a weight, in both. They go up to 2^15, so one is
+//    lost to f16's smallest number, 2^-24, only 2^36 below the largest.
 // 2. kv8_chunk_kernel: a CTA takes two 128-row query tiles (fp16: one and its remainder) of one (sequence, kv head) - rows of all the heads that
 //    share it, so a key tile is loaded once for them - and a range of the 128-key tiles. One thread feeds a ring of K
 //    and V tiles by TMA, one issues S = Q K^T and O += P V as tcgen05.mma with S and O in tensor memory, two
 //    warpgroups (thread = query row) turn S into weights: x = s * (factor * scale_k) + log2 scale_v for each 32 keys, w =
-//    2^(x - m), l += sum w / scale_v, P = f16(w) to shared memory. m moves only when a tile raises it by more than
-//    2^8. The scales cost nothing per score: the FMA of the softmax takes them as its factor and addend.
+//    2^(x - m + HEADROOM), l += sum w / scale_v, P = f16(w) to shared memory. m moves only when a tile raises it by more than
+//    2^4. The scales cost nothing per score: the FMA of the softmax takes them as its factor and addend.
 // 3. With the key axis split (few query tiles), kv8_join_kernel merges the parts in their order.
 // Bound by the softmax's latency: products and exponentials take some 2000 cycles each for a pair of tiles at D = 128, a
 // step some 6000 (8 softmax warps on 4 schedulers). 512 tokens of 32 heads of 128 at 7001: 129 us in all, 100 of them
@@ -39,7 +40,8 @@ constexpr int BKV = 128;
 constexpr int SOFTMAX_WARPS = 8;
 constexpr int TMA_WARP = 8, MMA_WARP = 9;
 constexpr int THREADS = 12 * 32;  // the last two warps only make up a warpgroup
-constexpr float LAZY_RESCALE_LOG2 = 8.f;
+constexpr float LAZY_RESCALE_LOG2 = 4.f;
+constexpr float HEADROOM = 11.f;  // log2 of a weight at the maximum; with what that may lag behind, 15: the top of f16
 
 template <int D>
 struct Smem {
@@ -246,14 +248,10 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32, 2) kv8_expand_kernel(const 
   }
   const uint32_t amax = amax2_warp(m);
   __syncwarp();
-  const float up = DT == TK_F16 ? 1.f : to_f16_range(amax << 16);
+  const float up = values ? value_factor<DT>(amax) : DT == TK_F16 ? 1.f : to_f16_range(amax << 16);
   auto to_half = [&](uint32_t w) -> uint32_t {
-    if constexpr (DT == TK_F16) {
-      return w;
-    } else {
-      const float2 v = unpack2<DT>(w);
-      return h2_u32(__floats2half2_rn(v.x * up, v.y * up));
-    }
+    const float2 v = unpack2<DT>(w);
+    return h2_u32(__floats2half2_rn(v.x * up, v.y * up));
   };
   if (!values) {
 #pragma unroll 4
@@ -491,7 +489,7 @@ __global__ void __launch_bounds__(THREADS, 1)
           m_use = mx;
           alpha = exp2_approx(m_run - mx);
         }
-        const float base = m_use == -INFINITY ? 0.f : m_use;  // no key of this row so far
+        const float base = m_use == -INFINITY ? 0.f : m_use - HEADROOM;  // no key of this row so far
         float rs = 0.f;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
