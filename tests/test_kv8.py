@@ -619,3 +619,39 @@ def test_small_weights_beside_a_dominant_token(dt, code, size, S, who, gap):
             tol += (2.0 ** -36 if once else 2.0 ** -40) * (200 if who == "first" else 1) * V.abs().sum(0)
             err = (out[b, :, h] - p @ V).abs()
             assert (err <= tol).all(), f"error / bound {(err / tol).max().item()}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 20, 40])  # 40: the tensor-core form
+@pytest.mark.parametrize("power", [60, 70, 110])
+@pytest.mark.parametrize("small", ["first", "middle", "open", "large first"])
+def test_blocks_of_zeros_beside_large_values(small, power, S):
+    """bf16 values of 2^60 and more beside blocks of zeros (whose scale is the least that there is): the weights of those
+    count in the denominator, in whatever order the blocks come and however they are split and merged."""
+    require_b200()
+    from tinker_b200.kernels import kv8_append, kv8_attention, kv8_dequantize, kv8_empty
+    B, hq, hkv, d, n = 2, 4, 2, 64, 1000
+    g = torch.Generator(device="cuda").manual_seed(S)
+    cache = kv8_empty(B, hkv, d, 1088, torch.bfloat16)
+    k = torch.randn(B, n, hkv * d, device="cuda", generator=g).bfloat16()
+    v = torch.randn(B, n, hkv * d, device="cuda", generator=g) * 2.0 ** power
+    vn = torch.randn(B, S, hkv * d, device="cuda", generator=g) * 2.0 ** power
+    if small == "first":
+        v[:, :640] = 0
+    elif small == "middle":
+        v[:, 320:352] = 0
+        v[:, 608:800] = 0
+    elif small == "open":
+        v[:, 992:] = 0
+        vn[:] = 0
+    else:
+        v[:, 32:] = 0
+    v, vn = v.bfloat16(), vn.bfloat16()
+    kv8_append(k, v, *cache, 0)
+    rows = [torch.cat([t.double() for t in kv8_dequantize(*(t[b:b + 1] for t in cache), n)]) for b in range(B)]
+    q = torch.randn(B, S, hq * d, device="cuda", generator=g).bfloat16()
+    kn = torch.randn(B, S, hkv * d, device="cuda", generator=g).bfloat16()
+    want, tol, _, _ = exact(q, kn, vn, None, None, rows, [n] * B, hq, hkv, d)
+    out = kv8_attention(q, kn, vn, None, None, *cache, hq, hkv, d, start_pos=n)
+    err = (out.double() - want).abs()
+    assert (err <= tol).all(), f"error / bound {(err / tol).max().item()}"

@@ -16,7 +16,11 @@
 //     w = 2^(x + log2 scale_v - m + HEADROOM), m the running maximum of x + log2 scale_v, O = sum w * code, and the
 //     softmax's denominator is sum w / scale_v. So O needs no pass per block, and the rounding of log2 scale_v cancels
 //     between numerator and denominator. w goes up to 2^15, the top of f16's range, so that a weight is lost to its
-//     smallest number, 2^-24, only 2^40 below the largest: a million of them are still 2^-20 of the result.
+//     smallest number, 2^-24, only 2^40 below the largest: a million of them are still 2^-20 of the result. With bf16 the
+//     scales of two blocks can be 2^188 apart (zeros beside values of 2^120), so w can leave fp32's range below while w /
+//     scale_v counts in the denominator: where a lane's keys are all 2^60 below m it takes their shares of the denominator
+//     as exponentials of their own, and sums of shares are scaled in two steps, by the root of the factor (an f16 cache's
+//     scales are 2^76 apart at most, so what is lost of w is below 2^-126 2^76 of the denominator).
 // (The keys as columns, with f16(q) and remainder as two halves of the 16 rows, took 274 instead of 231 instructions
 // for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 18.7 us for 64 sequences of 4
 // kv heads at 2047.)
@@ -131,8 +135,8 @@ struct Rows {
 // N tiles in one step (independent products and one maximum, so that a warp that has a scheduler to itself waits
 // less): key_words(u, j, h, w) and value_words(u, m, w) give the f16 pairs w[0..7] of the lane's fragment of tile u
 // (kv8.cuh), `sk` the factor of the raw products, `lsv` log2 of the values' scale, `isv` its inverse, allowed(g, token)
-// the mask. qf[g][k step] is the fragment of the query rows.
-template <int D, int NG, int N, bool MASK, typename KF, typename VF, typename AF>
+// the mask. qf[g][k step] is the fragment of the query rows. WIDE: the values' scales may lie far apart (bf16).
+template <int D, int NG, int N, bool MASK, bool WIDE, typename KF, typename VF, typename AF>
 __device__ __forceinline__ void attend_tiles(Rows<D, NG>& st, const uint32_t (&qf)[NG][D / 16][2],
                                              const float (&sk)[NG][N], const float (&lsv)[N], const float (&isv)[N],
                                              int lane, KF key_words, VF value_words, AF allowed) {
@@ -168,14 +172,16 @@ __device__ __forceinline__ void attend_tiles(Rows<D, NG>& st, const uint32_t (&q
         }
       }
     }
-  float mn[NG];
+  float mn[NG], own[NG][N];
   bool grown = false;
 #pragma unroll
   for (int g = 0; g < NG; ++g) {
     float mx = -INFINITY;
 #pragma unroll
-    for (int u = 0; u < N; ++u)
-      mx = fmaxf(mx, fmaxf(fmaxf(s[g][u][0], s[g][u][1]), fmaxf(s[g][u][2], s[g][u][3])));
+    for (int u = 0; u < N; ++u) {
+      own[g][u] = fmaxf(fmaxf(s[g][u][0], s[g][u][1]), fmaxf(s[g][u][2], s[g][u][3]));
+      mx = fmaxf(mx, own[g][u]);
+    }
 #pragma unroll
     for (int o = 4; o < 32; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
     mn[g] = fmaxf(st.m[g], mx);
@@ -185,8 +191,8 @@ __device__ __forceinline__ void attend_tiles(Rows<D, NG>& st, const uint32_t (&q
 #pragma unroll
     for (int g = 0; g < NG; ++g) {
       // O's columns are the rows' weights in two parts, in this lane those of row q: the factor is the lane's own
-      const float a = mn[g] == -INFINITY ? 1.f : exp2_approx(st.m[g] - mn[g]);
-      st.l[g] *= a;
+      const float root = mn[g] == -INFINITY ? 1.f : exp2_approx(0.5f * (st.m[g] - mn[g])), a = root * root;
+      st.l[g] = st.l[g] * root * root;
 #pragma unroll
       for (int n = 0; n < D / 16; ++n)
 #pragma unroll
@@ -207,7 +213,14 @@ __device__ __forceinline__ void attend_tiles(Rows<D, NG>& st, const uint32_t (&q
         sum += w;
         pf[g][j] = transpose8(h2_u32(__floats2half2_rn(w, w - __half2float(__float2half_rn(w)))));
       }
-      st.l[g] = fmaf(sum, isv[u], st.l[g]);
+      if (WIDE && own[g][u] < mn[g] - 60.f) {
+        sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) sum += exp2_approx((s[g][u][j] - lsv[u]) - base);
+        st.l[g] += sum;
+      } else {
+        st.l[g] = fmaf(sum, isv[u], st.l[g]);
+      }
     }
 #pragma unroll
     for (int n = 0; n < D / 16; ++n) {
@@ -291,8 +304,10 @@ struct Merged {
     for (int g = 0; g < NG; ++g) {
       const float mn = fmaxf(m[g], ml[g].x);
       const float base = mn == -INFINITY ? 0.f : mn;  // nothing but rows without a key so far
-      const float a = exp2_approx(m[g] - base), e = exp2_approx(ml[g].x - base);
-      l[g] = l[g] * a + ml[g].y * e;
+      // by the roots of the factors: a denominator can count where the factor itself is below fp32's range
+      const float ra = exp2_approx(0.5f * (m[g] - base)), re = exp2_approx(0.5f * (ml[g].x - base));
+      const float a = ra * ra, e = re * re;
+      l[g] = l[g] * ra * ra + ml[g].y * re * re;
 #pragma unroll
       for (int n = 0; n < D / 8; ++n) o[g][n] = o[g][n] * a + v[g][n] * e;
       m[g] = mn;
@@ -631,7 +646,7 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
 #pragma unroll
       for (int cg = 0; cg < NG; ++cg) sk1[cg][0] = cq[cg] / fk;
       const float lsv1[1] = {-__log2f(fv)}, isv1[1] = {fv};
-      attend_tiles<D, NG, 1, true>(
+      attend_tiles<D, NG, 1, true, DT == TK_BF16>(
           st, qf, sk1, lsv1, isv1, lane,
           [&](int, int jj, int h, uint32_t (&w)[8]) {
             const int row = 8 * (r >> 1) + 2 * jj + (r & 1);
@@ -703,7 +718,7 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
       const uint8_t* slot[N];
 #pragma unroll
       for (int u = 0; u < N; ++u) slot[u] = ring + ((j + u) % S::STAGES) * S::STAGE + lane * 16;
-      attend_tiles<D, NG, N, false>(
+      attend_tiles<D, NG, N, false, DT == TK_BF16>(
           st, qf, sk, lsv, isv, lane,
           [&](int u, int jj, int h, uint32_t (&w)[8]) {
             const uint4 x = *reinterpret_cast<const uint4*>(slot[u] + (jj * H + h) * 512);

@@ -26,6 +26,7 @@
 #include <algorithm>
 #include <cmath>
 #include <string>
+#include <type_traits>
 
 #include "kv8.cuh"
 #include "kv8_host.h"
@@ -95,6 +96,12 @@ struct Params {
 
 // fp16: a query tile's remainder takes the place of the second tile
 template <int DT> constexpr bool REMAINDER = DT == TK_F16;
+// The values' scales may lie so far apart that a weight is below fp32's range and its share of the denominator, weight /
+// scale_v, is not: see kv8_attention.cu. Here the shares of 32 keys whose scale is 2^SPREAD below the greatest are
+// exponentials of their own, in a loop that only CTAs with values of 2^20 and more take (a branch in the one loop cost
+// 3 %).
+template <int DT> constexpr bool WIDE = DT == TK_BF16;
+constexpr float SPREAD = 80.f, LSV_LOW = -69.f;  // the least log2 scale_v: 2^-60 / 448
 
 constexpr int EXPAND_WARPS = 8;  // 4 for keys, 4 for values
 
@@ -453,88 +460,108 @@ __global__ void __launch_bounds__(THREADS, 1)
       const int qpos = p.start + (valid ? row : p.rows - 1) / p.groups;
       const int rows16 = p.start / BLOCK * BLOCK;  // the first position that is kept in 16 bits; no row's own is below it
       const float4* sx = p.sx + bh * (p.keys / BLOCK) + static_cast<int64_t>(lo) * (BKV / BLOCK);
-      for (int j = 0; ok && j < n_x; ++j) {
-        float4 sc[4];  // from L1: one line holds two tiles' and the line after it is on its way
+      auto tiles = [&](auto wide, float top) {  // top: the greatest log2 scale_v of the CTA's keys
+        for (int j = 0; ok && j < n_x; ++j) {
+          float4 sc[4];  // from L1: one line holds two tiles' and the line after it is on its way
 #pragma unroll
-        for (int i = 0; i < 4; ++i) sc[i] = sx[4 * j + i];
-        if (lane == 0 && j + 3 < n_x) prefetch_l1(sx + 4 * (j + 3));
-        if (!mbar_wait(bars + B_S_FULL + x, j & 1)) { ok = false; break; }
-        tc_fence_after();
-        float sv[BKV];
-        tmem_load128(t_s + lane_off, sv);
-        tc_fence_before();
-        mbar_arrive(bars + B_S_FREE + x);
-        const int key = (lo + j) * BKV;
-        if (key + BKV > rows16) {  // the open block and the call's own tokens: the mask, and tokens that are NaN
-#pragma unroll
-          for (int c = 0; c < BKV; ++c) {
-            if (__float_as_uint(sc[c >> 5].w) >> (c & 31) & 1) sv[c] = __uint_as_float(0x7fc00000u);
-            if (key + c > qpos) sv[c] = -INFINITY;
-          }
-        }
-        // the maximum of x: for each 32 keys that of the raw products, times their factor
-        float f[4], mx = -INFINITY;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          float m2[2] = {sv[32 * i], sv[32 * i + 1]};
-#pragma unroll
-          for (int c = 2; c < 32; ++c) m2[c & 1] = fmaxf(m2[c & 1], sv[32 * i + c]);
-          f[i] = cq * sc[i].x;
-          if (f[i] < 1e-30f) f[i] = 1e-30f;  // not 0, which times a masked -inf is NaN
-          const float raw = fmaxf(m2[0], m2[1]);
-          mx = fmaxf(mx, fmaf(raw, f[i], sc[i].y));
-        }
-        float m_use = m_run, alpha = 1.f;
-        if (mx > m_run + LAZY_RESCALE_LOG2) {
-          m_use = mx;
-          alpha = exp2_approx(m_run - mx);
-        }
-        const float base = m_use == -INFINITY ? 0.f : m_use - HEADROOM;  // no key of this row so far
-        float rs = 0.f;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          const uint64_t f2 = pack_f32x2(f[i], f[i]), a2 = pack_f32x2(sc[i].y - base, sc[i].y - base);
-          uint64_t s2[2] = {0, 0};
-#pragma unroll
-          for (int c = 32 * i; c < 32 * i + 32; c += 2) {
-            float e0, e1;
-            unpack_f32x2(fma_f32x2(pack_f32x2(sv[c], sv[c + 1]), f2, a2), e0, e1);
-            sv[c] = exp2_approx(e0);
-            sv[c + 1] = exp2_approx(e1);
-            s2[(c >> 1) & 1] = add_f32x2(s2[(c >> 1) & 1], pack_f32x2(sv[c], sv[c + 1]));
-          }
-          float a, c2, d, e;
-          unpack_f32x2(s2[0], a, c2);
-          unpack_f32x2(s2[1], d, e);
-          rs = fmaf((a + c2) + (d + e), sc[i].z, rs);
-        }
-        l_run = l_run * alpha + rs;
-        m_run = m_use;
-        if (j > 0) {  // P and O are still in use by the P V before
-          if (!mbar_wait(bars + B_PV_DONE + x, (j - 1) & 1)) { ok = false; break; }
+          for (int i = 0; i < 4; ++i) sc[i] = sx[4 * j + i];
+          if (lane == 0 && j + 3 < n_x) prefetch_l1(sx + 4 * (j + 3));
+          if (!mbar_wait(bars + B_S_FULL + x, j & 1)) { ok = false; break; }
           tc_fence_after();
-        }
+          float sv[BKV];
+          tmem_load128(t_s + lane_off, sv);
+          tc_fence_before();
+          mbar_arrive(bars + B_S_FREE + x);
+          const int key = (lo + j) * BKV;
+          if (key + BKV > rows16) {  // the open block and the call's own tokens: the mask, and tokens that are NaN
 #pragma unroll
-        for (int c = 0; c < BKV / 8; ++c) {
-          uint32_t w[4];
-#pragma unroll
-          for (int i = 0; i < 4; ++i) w[i] = h2_u32(__floats2half2_rn(sv[c * 8 + 2 * i], sv[c * 8 + 2 * i + 1]));
-          *reinterpret_cast<uint4*>(sp + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) * 16)) =
-              make_uint4(w[0], w[1], w[2], w[3]);
-        }
-        if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
-#pragma unroll
-          for (int c = 0; c < D; c += 32) {
-            float o[32];
-            tmem_load32(t_o + lane_off + c, o);
-#pragma unroll
-            for (int i = 0; i < 32; ++i) o[i] *= alpha;
-            tmem_st32(t_o + lane_off + c, o);
+            for (int c = 0; c < BKV; ++c) {
+              if (__float_as_uint(sc[c >> 5].w) >> (c & 31) & 1) sv[c] = __uint_as_float(0x7fc00000u);
+              if (key + c > qpos) sv[c] = -INFINITY;
+            }
           }
+          // the maximum of x: for each 32 keys that of the raw products, times their factor
+          float f[4], mx = -INFINITY;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            float m2[2] = {sv[32 * i], sv[32 * i + 1]};
+#pragma unroll
+            for (int c = 2; c < 32; ++c) m2[c & 1] = fmaxf(m2[c & 1], sv[32 * i + c]);
+            f[i] = cq * sc[i].x;
+            if (f[i] < 1e-30f) f[i] = 1e-30f;  // not 0, which times a masked -inf is NaN
+            const float raw = fmaxf(m2[0], m2[1]);
+            mx = fmaxf(mx, fmaf(raw, f[i], sc[i].y));
+          }
+          float m_use = m_run, root = 1.f, alpha = 1.f;
+          if (mx > m_run + LAZY_RESCALE_LOG2) {
+            m_use = mx;
+            if constexpr (WIDE<DT>) root = exp2_approx(0.5f * (m_run - mx));
+            alpha = WIDE<DT> ? root * root : exp2_approx(m_run - mx);
+          }
+          const float base = m_use == -INFINITY ? 0.f : m_use - HEADROOM;  // no key of this row so far
+          float rs = 0.f;
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            if constexpr (decltype(wide)::value) {
+              if (sc[i].y < top - SPREAD) {
+#pragma unroll
+                for (int c = 32 * i; c < 32 * i + 32; ++c) rs += exp2_approx(fmaf(sv[c], f[i], -base));
+                sc[i].z = 0.f;
+              }
+            }
+            const uint64_t f2 = pack_f32x2(f[i], f[i]), a2 = pack_f32x2(sc[i].y - base, sc[i].y - base);
+            uint64_t s2[2] = {0, 0};
+#pragma unroll
+            for (int c = 32 * i; c < 32 * i + 32; c += 2) {
+              float e0, e1;
+              unpack_f32x2(fma_f32x2(pack_f32x2(sv[c], sv[c + 1]), f2, a2), e0, e1);
+              sv[c] = exp2_approx(e0);
+              sv[c + 1] = exp2_approx(e1);
+              s2[(c >> 1) & 1] = add_f32x2(s2[(c >> 1) & 1], pack_f32x2(sv[c], sv[c + 1]));
+            }
+            float a, c2, d, e;
+            unpack_f32x2(s2[0], a, c2);
+            unpack_f32x2(s2[1], d, e);
+            rs = fmaf((a + c2) + (d + e), sc[i].z, rs);
+          }
+          l_run = (WIDE<DT> ? l_run * root * root : l_run * alpha) + rs;
+          m_run = m_use;
+          if (j > 0) {  // P and O are still in use by the P V before
+            if (!mbar_wait(bars + B_PV_DONE + x, (j - 1) & 1)) { ok = false; break; }
+            tc_fence_after();
+          }
+#pragma unroll
+          for (int c = 0; c < BKV / 8; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) w[i] = h2_u32(__floats2half2_rn(sv[c * 8 + 2 * i], sv[c * 8 + 2 * i + 1]));
+            *reinterpret_cast<uint4*>(sp + (c >> 3) * (128 * 128) + r * 128 + (((c & 7) ^ (r & 7)) * 16)) =
+                make_uint4(w[0], w[1], w[2], w[3]);
+          }
+          if (j > 0 && __any_sync(0xffffffffu, alpha != 1.0f)) {
+#pragma unroll
+            for (int c = 0; c < D; c += 32) {
+              float o[32];
+              tmem_load32(t_o + lane_off + c, o);
+#pragma unroll
+              for (int i = 0; i < 32; ++i) o[i] *= alpha;
+              tmem_st32(t_o + lane_off + c, o);
+            }
+          }
+          fence_proxy_async_smem();
+          tc_fence_before();
+          mbar_arrive(bars + B_P_FULL + x);
         }
-        fence_proxy_async_smem();
-        tc_fence_before();
-        mbar_arrive(bars + B_P_FULL + x);
+      };
+      if constexpr (WIDE<DT>) {
+        float top = -INFINITY;
+        for (int i = lane; i < n_x * (BKV / BLOCK); i += 32) top = fmaxf(top, sx[i].y);
+#pragma unroll
+        for (int o = 16; o > 0; o >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, o));
+        if (top > LSV_LOW + SPREAD) tiles(std::true_type(), top);
+        else tiles(std::false_type(), top);
+      } else {
+        tiles(std::false_type(), 0.f);
       }
       const int64_t slot = (bh * p.rows + row) * p.splits + split;
       if (ok && n_x > 0) ok = mbar_wait(bars + B_PV_DONE + x, (n_x - 1) & 1);
@@ -595,8 +622,8 @@ __global__ void __launch_bounds__(256) kv8_join_kernel(const Params p) {
     const float2 ml = __ldcg(p.part_ml + slot + i);
     if (ml.x == -INFINITY && ml.y == 0.f) continue;  // no key of this row in the part
     const float mn = fmaxf(M, ml.x);
-    const float a = exp2_approx(M - mn), e = exp2_approx(ml.x - mn);
-    L = L * a + ml.y * e;
+    const float ra = exp2_approx(0.5f * (M - mn)), re = exp2_approx(0.5f * (ml.x - mn)), a = ra * ra, e = re * re;
+    L = L * ra * ra + ml.y * re * re;
     if constexpr (E == 4) {
       const float4 o = __ldcg(reinterpret_cast<const float4*>(from + static_cast<int64_t>(i) * D));
       acc[0] = acc[0] * a + o.x * e;
