@@ -655,3 +655,58 @@ def test_blocks_of_zeros_beside_large_values(small, power, S):
     out = kv8_attention(q, kn, vn, None, None, *cache, hq, hkv, d, start_pos=n)
     err = (out.double() - want).abs()
     assert (err <= tol).all(), f"error / bound {(err / tol).max().item()}"
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [9, 40])  # 18 and 80 query rows of a kv head: the one form and the other
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("power", [-40, 20])
+def test_a_token_that_is_not_finite_leaves_the_others_their_range(power, bad, what, S):
+    """bf16 keys and values outside f16's range beside a token that is not finite, in the same 32 tokens: the rows before
+    it are what they are without it."""
+    require_b200()
+    from tinker_b200.kernels import kv8_append, kv8_attention, kv8_dequantize, kv8_empty
+    B, hq, hkv, d, n, at = 2, 8, 4, 64, 130, 6
+    g = torch.Generator(device="cuda").manual_seed(S)
+    cache = kv8_empty(B, hkv, d, 256, torch.bfloat16)
+    k, v = ((torch.randn(B, n, hkv * d, device="cuda", generator=g) * 2.0 ** power).bfloat16() for _ in range(2))
+    kv8_append(k, v, *cache, 0)
+    rows = [torch.cat([t.double() for t in kv8_dequantize(*(t[b:b + 1] for t in cache), n)]) for b in range(B)]
+    q = (torch.randn(B, S, hq * d, device="cuda", generator=g) * 2.0 ** -power).bfloat16()
+    kn, vn = ((torch.randn(B, S, hkv * d, device="cuda", generator=g) * 2.0 ** power).bfloat16() for _ in range(2))
+    want, tol, _, _ = exact(q, kn, vn, None, None, rows, [n] * B, hq, hkv, d)
+    (kn if what == "k" else vn)[0, at, d + 3] = bad  # sequence 0, kv head 1: heads 2 and 3
+    out = kv8_attention(q, kn, vn, None, None, *cache, hq, hkv, d, start_pos=n).double()
+    seen = torch.zeros(B, S, hq * d, dtype=torch.bool, device="cuda")
+    seen[0, at:, 2 * d:4 * d] = True
+    assert torch.isnan(out[seen]).all()
+    assert ((out - want).abs() <= tol)[~seen].all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["fp16", "bf16"])
+@pytest.mark.parametrize("what", ["k", "v"])
+@pytest.mark.parametrize("bad", [math.nan, math.inf, -math.inf])
+@pytest.mark.parametrize("S, n", [(1, 70), (1, 95), (3, 70), (40, 70)])
+def test_rows_that_see_a_token_that_is_not_finite_are_nan(S, n, bad, what, dt):
+    """In every form, and as they are once the token's block is complete; other heads and sequences are not."""
+    require_b200()
+    from tinker_b200.kernels import kv8_append, kv8_attention, kv8_empty
+    dtype, B, hq, hkv, d = DTYPES[dt], 2, 8, 4, 64
+    g = torch.Generator(device="cuda").manual_seed(n)
+    for where in ("open", "own"):
+        cache = kv8_empty(B, hkv, d, 160, dtype)
+        k, v = (torch.randn(B, n, hkv * d, device="cuda", generator=g).to(dtype) for _ in range(2))
+        q, kn, vn = (torch.randn(B, S, h * d, device="cuda", generator=g).to(dtype) for h in (hq, hkv, hkv))
+        if where == "open":
+            (k if what == "k" else v)[0, n - 2, d + 3] = bad  # sequence 0, kv head 1: heads 2 and 3
+        else:
+            (kn if what == "k" else vn)[0, S - 1, d + 3] = bad
+        kv8_append(k, v, *cache, 0)
+        out = kv8_attention(q, kn, vn, None, None, *cache, hq, hkv, d, start_pos=n)
+        seen = torch.zeros(B, S, hq * d, dtype=torch.bool, device="cuda")
+        seen[0, 0 if where == "open" else S - 1:, 2 * d:4 * d] = True
+        assert torch.isnan(out[seen]).all() and torch.isfinite(out[~seen]).all()
+        nxt = kv8_attention(q[:, :1], k[:, :1], v[:, :1], None, None, *cache, hq, hkv, d, start_pos=n + S)
+        assert torch.isnan(nxt[0, :, 2 * d:4 * d]).all() and torch.isfinite(nxt[1]).all()

@@ -74,10 +74,16 @@ __device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) 
   }
 }
 
+// The least pattern of a magnitude that is infinite or NaN.
+template <int DT>
+__device__ __forceinline__ constexpr uint32_t not_finite_bits() {
+  return DT == TK_F16 ? 0x7c00u : 0x7f80u;
+}
+
 // Scale of a block from the 16-bit pattern of its largest magnitude; `inv` is what its values are multiplied by.
 template <int DT, int FMT>
 __device__ __forceinline__ float block_scale(uint32_t amax_bits, float& inv) {
-  const bool fine = amax_bits < (DT == TK_F16 ? 0x7c00u : 0x7f80u);
+  const bool fine = amax_bits < not_finite_bits<DT>();
   const unsigned short b = static_cast<unsigned short>(amax_bits);
   float a;
   if constexpr (DT == TK_F16) a = __half2float(__ushort_as_half(b));
@@ -139,7 +145,7 @@ __device__ __forceinline__ uint32_t amax2_warp(uint32_t m) {
 template <int DT>
 __device__ __forceinline__ bool not_finite(uint4 x) {
   const uint32_t m = amax2(amax2(amax2(amax2(0u, x.x), x.y), x.z), x.w);
-  return max(m & 0xffffu, m >> 16) >= (DT == TK_F16 ? 0x7c00u : 0x7f80u);
+  return max(m & 0xffffu, m >> 16) >= not_finite_bits<DT>();
 }
 
 // A warp's 16-bit tile in shared memory: 32 rows of D elements in 16-byte chunks, chunk c of row t at c ^ swz(t),

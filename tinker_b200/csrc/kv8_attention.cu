@@ -603,26 +603,6 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
       }
       __syncwarp();
       uint32_t km = 0, vm = 0;
-      if (p.seq > 1) {
-        // Values that are not finite must not reach the rows that do not see their token (0 * NaN): the token's key
-        // becomes NaN, which the mask hides from those rows and which makes the others NaN, and its values 0.
-        uint32_t bad = 0;
-#pragma unroll 1
-        for (int idx = lane; idx < BLOCK * C16; idx += 32)
-          if (not_finite<DT>(*reinterpret_cast<const uint4*>(vtile + tile_off<D>(idx / C16, idx % C16))))
-            bad |= 1u << (idx / C16);
-        bad = __reduce_or_sync(0xffffffffu, bad);
-        if (bad) {
-#pragma unroll 1
-          for (int idx = lane; idx < BLOCK * C16; idx += 32) {
-            if (!(bad >> (idx / C16) & 1)) continue;
-            const uint32_t off = tile_off<D>(idx / C16, idx % C16);
-            *reinterpret_cast<uint4*>(ktile + off) = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
-            *reinterpret_cast<uint4*>(vtile + off) = make_uint4(0, 0, 0, 0);
-          }
-          __syncwarp();
-        }
-      }
 #pragma unroll 4
       for (int i = 0; i < C16; ++i) {  // any order of the tile's chunks
         const uint4 kx = *reinterpret_cast<const uint4*>(ktile + (lane + 32 * i) * 16);
@@ -632,6 +612,37 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
       }
       km = amax2_warp(km);
       vm = amax2_warp(vm);
+      // A token that is not finite makes the rows that see it NaN: its scores are. One token's rows see all of the tile.
+      const bool broken = max(km, vm) >= not_finite_bits<DT>();
+      if (broken && p.seq > 1) {
+        // It must not reach the rows that do not see it, neither as 0 * NaN nor by the tile's range: its key becomes NaN,
+        // which the mask hides from those rows, its values 0.
+        uint32_t bad = 0;
+#pragma unroll 1
+        for (int idx = lane; idx < BLOCK * C16; idx += 32) {
+          const uint32_t off = tile_off<D>(idx / C16, idx % C16);
+          if (not_finite<DT>(*reinterpret_cast<const uint4*>(ktile + off)) ||
+              not_finite<DT>(*reinterpret_cast<const uint4*>(vtile + off)))
+            bad |= 1u << (idx / C16);
+        }
+        bad = __reduce_or_sync(0xffffffffu, bad);
+        km = vm = 0;
+#pragma unroll 1
+        for (int idx = lane; idx < BLOCK * C16; idx += 32) {
+          uint4* kx = reinterpret_cast<uint4*>(ktile + tile_off<D>(idx / C16, idx % C16));
+          uint4* vx = reinterpret_cast<uint4*>(vtile + tile_off<D>(idx / C16, idx % C16));
+          if (bad >> (idx / C16) & 1) {
+            *kx = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+            *vx = make_uint4(0, 0, 0, 0);
+          } else {
+            km = amax2(amax2(amax2(amax2(km, kx->x), kx->y), kx->z), kx->w);
+            vm = amax2(amax2(amax2(amax2(vm, vx->x), vx->y), vx->z), vx->w);
+          }
+        }
+        km = amax2_warp(km);
+        vm = amax2_warp(vm);
+        __syncwarp();
+      }
 
       const float fk = DT == TK_F16 ? 1.f : to_f16_range(km << 16), fv = value_factor<DT>(vm);
       auto to_half = [](uint32_t w, float f) -> uint32_t {
@@ -644,7 +655,8 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
       };
       float sk1[NG][1];
 #pragma unroll
-      for (int cg = 0; cg < NG; ++cg) sk1[cg][0] = cq[cg] / fk;
+      for (int cg = 0; cg < NG; ++cg)
+        sk1[cg][0] = broken && p.seq == 1 ? __uint_as_float(0x7fc00000u) : cq[cg] / fk;
       const float lsv1[1] = {-__log2f(fv)}, isv1[1] = {fv};
       attend_tiles<D, NG, 1, true, DT == TK_BF16>(
           st, qf, sk1, lsv1, isv1, lane,

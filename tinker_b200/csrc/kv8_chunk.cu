@@ -226,7 +226,7 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32, 2) kv8_expand_kernel(const 
   const int64_t stride = values ? p.vs : p.ks;
   const int row0 = (block - n8) * BLOCK - open;  // the call's row of the block's first token
   uint8_t* tile = smem + warp * (BLOCK * D * 2);
-  uint32_t m = 0, bad = 0;
+  uint32_t m = 0;
   uint4 x[C16];
 #pragma unroll
   for (int i = 0; i < C16; ++i) {  // all loads in flight, then the rotations
@@ -241,20 +241,29 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32, 2) kv8_expand_kernel(const 
       const int64_t ang = (static_cast<int64_t>(p.start) + s) * (D / 2) + c * 4;
       rope_chunk<DT>(x[i], p.cos_t + ang, p.sin_t + ang);
     }
-    if (values && not_finite<DT>(x[i])) bad |= 1u << t;
-  }
-  // A token whose values are not finite must not reach the rows that do not see it (0 * NaN): its values become 0, and
-  // the rows that see it NaN by its scores.
-  bad = __reduce_or_sync(0xffffffffu, bad);
-#pragma unroll
-  for (int i = 0; i < C16; ++i) {
-    const int idx = lane + 32 * i, t = idx / C16, c = idx % C16;
-    if (bad >> t & 1) x[i] = make_uint4(0, 0, 0, 0);
     m = amax2(amax2(amax2(amax2(m, x[i].x), x[i].y), x[i].z), x[i].w);
     *reinterpret_cast<uint4*>(tile + tile_off<D>(t, c)) = x[i];
   }
-  const uint32_t amax = amax2_warp(m);
+  uint32_t amax = amax2_warp(m), bad = 0;
   __syncwarp();
+  if (amax >= not_finite_bits<DT>()) {
+    // A token that is not finite makes the rows that see it NaN, by its scores, and must not reach the others, neither as 0 *
+    // NaN nor by the range of its 32 tokens: a key becomes NaN throughout, values become 0 and their bit does the same.
+#pragma unroll 1
+    for (int idx = lane; idx < BLOCK * C16; idx += 32)
+      if (not_finite<DT>(*reinterpret_cast<const uint4*>(tile + tile_off<D>(idx / C16, idx % C16)))) bad |= 1u << (idx / C16);
+    bad = __reduce_or_sync(0xffffffffu, bad);
+    const uint32_t w = values ? 0u : 0x7fff7fffu;
+    m = 0;
+#pragma unroll 1
+    for (int idx = lane; idx < BLOCK * C16; idx += 32) {
+      uint4* y = reinterpret_cast<uint4*>(tile + tile_off<D>(idx / C16, idx % C16));
+      if (bad >> (idx / C16) & 1) *y = make_uint4(w, w, w, w);
+      else m = amax2(amax2(amax2(amax2(m, y->x), y->y), y->z), y->w);
+    }
+    amax = amax2_warp(m);
+    __syncwarp();
+  }
   const float up = values ? value_factor<DT>(amax) : DT == TK_F16 ? 1.f : to_f16_range(amax << 16);
   auto to_half = [&](uint32_t w) -> uint32_t {
     const float2 v = unpack2<DT>(w);
