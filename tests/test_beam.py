@@ -361,3 +361,30 @@ def test_short_last_chunks_and_scattered_masks(V, n, dt):
     masked[0, 1] = low
     masked[0, 1, 100:103] = 1.0
     check(masked, scores, n)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt", ["bf16", "fp32"])
+@pytest.mark.parametrize("B, K, V", [(2, 4, 20011), (1, 3, 700), (60, 10, 50021)])  # the last one streams
+def test_finite_logits_of_any_magnitude(B, K, V, dt):
+    """One logit far above the others, up to the type's largest: its token at its beam's score, whatever the magnitude and
+    wherever it lies; and whole rows far below zero."""
+    require_b200()
+    from tinker_b200.kernels import beam_select
+    dtype = DTYPES[dt]
+    g = torch.Generator(device="cuda").manual_seed(V)
+    top = torch.finfo(dtype).max
+    for size in (1e6, 3e9, 1e10, 7e14, 1e30, 2.5e38, top):
+        logits = (torch.randn(B, K, V, device="cuda", generator=g) * 2).to(dtype)
+        at = torch.randint(0, V, (B, K), device="cuda", generator=g)
+        at[:, 0] = 3  # among the first elements
+        logits.scatter_(2, at[..., None], torch.full((B, K, 1), size, device="cuda", dtype=torch.float64).to(dtype))
+        scores = -torch.rand(B, K, device="cuda", generator=g).cumsum(1)
+        got, beams, tokens = beam_select(logits, scores, K)
+        assert torch.equal(tokens, at)
+        assert ((got.double() - scores.double()).abs() <= NEAR + 2.0 ** -24 * scores.double().abs()).all()  # log 1, as above
+        assert torch.equal(beams, torch.arange(K, device="cuda").expand(B, K))
+    low = (torch.randn(B, K, V, device="cuda", generator=g) * 2).to(dtype)
+    low[:, 1] = -3e9
+    low[:, 2] = -1e30
+    check(low, torch.zeros(B, K, device="cuda"), 4)

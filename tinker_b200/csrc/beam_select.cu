@@ -17,8 +17,8 @@
 //      the value of the n-th best so far; vectors that hold a larger one are put aside and, every STRIDE vectors,
 //      ranked with the best n, which raises the threshold. Equal elements that come later lose in any case.
 //      An exponential is 2^(x L - b) with L = log2 e and b = m L rounded; the sum is corrected by 2^(b - m L), the
-//      rounding that all its terms share. Where the reference proves too far off (a masked beginning), the sum is
-//      taken again. A segment with a NaN or +inf, or with more candidates than the lists hold, is done again in the
+//      rounding that all its terms share. Where the reference proves too far off (a masked beginning) or is above 2^20 (the
+//      rounding grows with it), the sum is taken again. A segment with a NaN or +inf, or with more candidates than the lists hold, is done again in the
 //      plain way: cleaned, its maximum, the sum of e^(x - m), n rounds of a maximum over (value, index).
 //   2. a CTA for each sequence joins the segments' sums to a logsumexp for each beam, takes a threshold from the heads of
 //      the segments' lists in the same way, walks each list down to it and ranks what it finds, with c in fp64.
@@ -477,7 +477,9 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
   }
   if (best == -INFINITY) {
     ref = -INFINITY;
-  } else if (sum == INFINITY || best < ref - 60.f) {  // the reference was too far off: once more with the maximum
+  } else if (sum == INFINITY || best < ref - 60.f || fabsf(ref) > 0x1p20f) {
+    // The reference was too far off, or so large that the rounding of b alone takes the terms out of fp32's range (ref L
+    // beyond 2^30: half a step of b is 64): once more with the maximum, subtracted before the product.
     sum = 0.f;
 #pragma unroll 1
     for (int at = lo + tid * VE; at < hi; at += STEP) {
