@@ -710,3 +710,27 @@ def test_rows_that_see_a_token_that_is_not_finite_are_nan(S, n, bad, what, dt):
         assert torch.isnan(out[seen]).all() and torch.isfinite(out[~seen]).all()
         nxt = kv8_attention(q[:, :1], k[:, :1], v[:, :1], None, None, *cache, hq, hkv, d, start_pos=n + S)
         assert torch.isnan(nxt[0, :, 2 * d:4 * d]).all() and torch.isfinite(nxt[1]).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt, code, B, hq, hkv, d, n", [("fp16", "e4m3", 1, 64, 1, 64, 500), ("bf16", "int8", 3, 71, 1, 64, 63),
+                                                        ("bf16", "e4m3", 2, 128, 2, 128, 130)])
+def test_one_token_of_many_heads(dt, code, B, hq, hkv, d, n):
+    """64 and more query heads for a kv head, one new token, the position on the host or on the device."""
+    require_b200()
+    from tinker_b200 import _lib
+    from tinker_b200.kernels import kv8_attention, kv8_attention_workspace
+    dtype = DTYPES[dt]
+    g = torch.Generator(device="cuda").manual_seed(n)
+    kc, vc, sc, tail, rows = make_cache(B, hkv, d, n + 1, [n] * B, dtype, code, g)
+    w = torch.randn(B, 1, (hq + 2 * hkv) * d, device="cuda", generator=g).to(dtype)
+    q, k, v = w.split([hq * d, hkv * d, hkv * d], -1)
+    want, tol, _, _ = exact(q, k, v, None, None, rows, [n] * B, hq, hkv, d, on_host=False)
+    ws = torch.zeros(kv8_attention_workspace(B, hq, hkv, d, 1, n + 1), dtype=torch.uint8, device="cuda")
+    for kw in (dict(start_pos=n), dict(start_pos=n, workspace=ws),
+               dict(position=torch.tensor([n], dtype=torch.int32, device="cuda"))):
+        cache = [t.clone() for t in (kc, vc, sc, tail)]
+        n0 = _lib.launch_counter[0]
+        out = kv8_attention(q, k, v, None, None, *cache, hq, hkv, d, **kw)
+        assert _lib.launch_counter[0] - n0 == 1
+        assert ((out.double() - want).abs() <= tol).all()

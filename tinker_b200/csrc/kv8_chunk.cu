@@ -742,9 +742,10 @@ static int sequences_at_once(int batch, int num_kv_heads, int64_t rows, int64_t 
   return static_cast<int>(std::max<int64_t>(1, std::min<int64_t>(batch, (int64_t(1) << 30) / std::max<int64_t>(one, 1))));
 }
 
+// One new token never: laying out the whole cache costs more than its step, and that one appends as it goes.
 bool chunk_fits(int batch, int num_heads, int num_kv_heads, int seq, int64_t len) {
   const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
-  return rows >= CHUNK_MIN_ROWS && rows < (1 << 20) && len < (1 << 30) && batch <= 65535 &&
+  return seq > 1 && rows >= CHUNK_MIN_ROWS && rows < (1 << 20) && len < (1 << 30) && batch <= 65535 &&
          int64_t(batch) * num_kv_heads < (1 << 30);
 }
 

@@ -27,7 +27,7 @@ int append(const Cache& c, const void* k, int64_t ks, const void* v, int64_t vs,
            const int* start_dev, int start_step, int dtype, cudaStream_t st);
 
 // The tensor-core form for many query rows (kv8_chunk.cu); appends nothing.
-constexpr int CHUNK_MIN_ROWS = 64;  // query rows of a kv head
+constexpr int CHUNK_MIN_ROWS = 64;  // query rows of a kv head, of two new tokens or more
 bool chunk_fits(int batch, int num_heads, int num_kv_heads, int seq, int64_t len);
 int64_t chunk_workspace(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int64_t len, int sm_count);
 int chunk_attention(const Cache& c, const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs,
