@@ -221,9 +221,9 @@ TK_API int tk_kv8_append(const void* k, int64_t k_tok_stride, const void* v, int
  * start_pos+S-1 against complete blocks (codes), the open block and their own rows (16 bits), then
  * their append. cos_table / sin_table NULL: q and k are rotated already. start_pos_device: the
  * position of sequence b is start_pos_device[b * start_pos_step] (step 0 or 1), read at run time; a
- * position outside the cache or the table records device error 2 and leaves that sequence's out
- * and cache as they are. A row that sees a token whose key or value holds a NaN or an infinity is NaN
- * throughout; other rows are what they are without it. workspace: tk_kv8_attention_workspace() bytes, zero-filled; calls of any
+ * position outside the cache or the table records device error 2, leaves that sequence's cache as it
+ * is and fills its rows of out with NaN. A row that sees a token whose key or value holds a NaN or an
+ * infinity is NaN throughout; other rows are what they are without it. workspace: tk_kv8_attention_workspace() bytes, zero-filled; calls of any
  * shape that follow one another on a stream can share it, calls that overlap must not. One launch for
  * S = 1, two otherwise; from 64 query rows of a kv head on, at a position known on the host, four or
  * more (the operands are laid out for the tensor cores first, in the workspace).

@@ -734,3 +734,35 @@ def test_one_token_of_many_heads(dt, code, B, hq, hkv, d, n):
         out = kv8_attention(q, k, v, None, None, *cache, hq, hkv, d, **kw)
         assert _lib.launch_counter[0] - n0 == 1
         assert ((out.double() - want).abs() <= tol).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+@pytest.mark.parametrize("S", [1, 3])
+@pytest.mark.parametrize("ragged", [True, False])
+def test_rows_of_a_position_outside_the_cache_are_nan(ragged, S, d):
+    """They are what the call returns for that sequence, not whatever was in memory."""
+    require_b200()
+    from tinker_b200 import _lib
+    from tinker_b200.kernels import kv8_attention
+    B, hq, hkv, cap = 300, 8, 2, 64
+    g = torch.Generator(device="cuda").manual_seed(9)
+    cache = make_cache(B, hkv, d, cap, [10] * B, torch.float16, "int8", g, garbage=False)[:4]
+    q, k, v = (torch.randn(B, S, h * d, device="cuda", generator=g).half() for h in (hq, hkv, hkv))
+    pos = torch.full((B,), 10, dtype=torch.int32, device="cuda")
+    pos[[0, 7, 299]] = torch.tensor([-1, cap - S + 1, 1 << 30], dtype=torch.int32, device="cuda")
+    if not ragged:
+        pos = pos[7:8].clone()
+    was = [t.clone() for t in cache]
+    _lib.device_error(clear=True)
+    torch.empty(B * S * hq * d, dtype=torch.float16, device="cuda").fill_(1.0)  # what the rows may be made of
+    out = kv8_attention(q, k, v, None, None, *cache, hq, hkv, d, position=pos)
+    torch.cuda.synchronize()
+    assert _lib.device_error(clear=True) == 2
+    bad = torch.zeros(B, dtype=torch.bool, device="cuda")
+    bad[[0, 7, 299]] = True
+    if not ragged:
+        bad[:] = True
+    assert torch.isnan(out[bad]).all() and torch.isfinite(out[~bad]).all()
+    for t, o in zip(cache, was):
+        assert torch.equal(t[bad].view(torch.uint8), o[bad].view(torch.uint8))

@@ -268,7 +268,7 @@ __device__ __forceinline__ int unit_weight(int start, int seq, int step) {
   return step == 1 ? w : quotient(w + step - 1, step) * step;
 }
 
-// A position that does not fit gives -1 (no weight): its sequence is left as it is.
+// A position that does not fit gives -1 (no weight): its sequence is left out.
 __device__ __forceinline__ int position_of(const AttnParams& p, int b) {
   const int start = p.start_dev ? __ldcg(p.start_dev + static_cast<int64_t>(b) * p.start_step) : p.start_pos;
   const int64_t end = static_cast<int64_t>(start) + p.seq;
@@ -375,7 +375,16 @@ __global__ void __launch_bounds__(THREADS, Smem<D, NG>::CTAS_SM) kv8_attention_k
     piece = whole ? PIECE_MIN : (exact + ctas * WARPS - 1) / (ctas * WARPS);
     step = whole ? WARPS * PIECE_MIN : 1;
   }
-  if (bad && me == 0) record_device_error(TK_DEVERR_POSITION);
+  if (__any_sync(0xffffffffu, bad)) {
+    if (me == 0) record_device_error(TK_DEVERR_POSITION);
+    // a sequence that is left out gives rows of NaN
+    const int row_chunks = p.num_kv_heads * p.groups * C16;
+    for (int64_t row = me; row < static_cast<int64_t>(p.batch) * p.seq; row += static_cast<int64_t>(ctas) * WARPS) {
+      if (position_of(p, static_cast<int>(row / p.seq)) >= 0) continue;
+      uint4* dst = reinterpret_cast<uint4*>(reinterpret_cast<T*>(p.out) + row * p.os);
+      for (int c = lane; c < row_chunks; c += 32) dst[c] = make_uint4(0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu, 0x7fff7fffu);
+    }
+  }
   if (static_cast<int64_t>(piece) * (blockIdx.x * WARPS) >= total) return;  // nothing for the whole CTA
   const int from = static_cast<int>(min(static_cast<int64_t>(piece) * me, static_cast<int64_t>(total)));
   const int to = static_cast<int>(min(static_cast<int64_t>(from) + piece, static_cast<int64_t>(total)));

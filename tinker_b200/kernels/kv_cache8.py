@@ -114,7 +114,7 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
     None when q and k are rotated already. The new tokens sit at ``start_pos ..``, or from
     ``position`` on, an int32 CUDA tensor of one element or of one per sequence that is read when the
     kernel runs (one CUDA graph serves every step); a position outside the cache or the tables then
-    records device error 2 and leaves that sequence's rows and cache untouched. Keys of complete blocks
+    records device error 2, leaves that sequence's cache untouched and gives rows of NaN for it. Keys of complete blocks
     are read as ``code * scale``, those of the open block and of this call in 16 bits. A row that sees a
     token whose key or value holds a NaN or an infinity is NaN throughout. ``workspace``:
     zero-filled uint8 CUDA tensor of at least ``kv8_attention_workspace(...)`` bytes, left so that
