@@ -145,3 +145,26 @@ def test_beam_search_is_the_exhaustive_search_when_wide():
     assert ((seqs == 4) | (ended == 0)).all()  # only the end token follows an end token
     assert torch.isfinite(scores).all() and not math.isnan(scores.sum().item())
     assert dec.beam_search(prompt, 25, 0)[0].shape == (2, 25, 0)
+
+
+@pytest.mark.gpu
+def test_beam_search_and_the_capacity():
+    """A search that cannot fit is refused before it begins, and leaves the decoder as it was; one that may end early runs
+    as far as the cache goes."""
+    require_b200()
+    import tinker_b200
+    from bench_model import make_tokens
+    cfg, _, model = _decoder(1)
+    prompt = make_tokens(cfg, 1, 30, seed=7).cuda()
+    dec = tinker_b200.CachedDecoder(model, batch_size=3, capacity=40)
+    full, scores = dec.beam_search(prompt, 3, 11)  # 30 + 11 - 1 positions
+    assert full.shape == (1, 3, 11) and dec.length == 40
+    with pytest.raises(ValueError, match="capacity 40"):
+        dec.beam_search(prompt, 3, 12)
+    assert dec.length == 40  # nothing ran
+    with pytest.raises(ValueError, match="capacity 40"):
+        dec.beam_search(make_tokens(cfg, 1, 41, seed=7), 3, 1, eos_token_id=1)
+    assert dec.beam_search(make_tokens(cfg, 1, 60, seed=7), 3, 0)[0].shape == (1, 3, 0)  # nothing to place
+    ends = int(next(t for t in range(cfg.vocab_size) if not (full == t).any()))  # never chosen, so no beam ends
+    seqs, got = dec.beam_search(prompt, 3, 50, eos_token_id=ends)
+    assert torch.equal(seqs, full) and torch.equal(got, scores)

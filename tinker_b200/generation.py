@@ -431,14 +431,21 @@ class CachedDecoder:
 
         Each step keeps the ``num_beams`` best continuations of every prompt by the sum of their
         log-probabilities; a beam that has produced ``eos_token_id`` keeps its score and is continued by
-        that token alone. Returns ``(tokens, scores)``: new token ids [prompts, num_beams, n] (CPU), best
-        beam first, n <= max_new_tokens (fewer once all beams have ended), and float32 scores [prompts,
+        that token alone. The prompt and all new tokens but the last need a place in the cache; with an
+        ``eos_token_id`` a search that may end early is begun all the same, and ends where the cache does.
+        Returns ``(tokens, scores)``: new token ids [prompts, num_beams, n] (CPU), best beam first, n <=
+        max_new_tokens (fewer once all beams have ended or the cache is full), and float32 scores [prompts,
         num_beams], the sum of log-probabilities divided by the number of tokens up to and including the end
         token to the power ``length_penalty``."""
         if prompt.dim() != 2 or num_beams < 1 or prompt.shape[0] * num_beams != self.batch_size:
             raise ValueError(f"prompt must be [prompts, S] with prompts * num_beams = {self.batch_size}")
         if num_beams > 32:
             raise ValueError("at most 32 beams")
+        room = self.capacity - prompt.shape[1] + 1  # tokens until the cache is full
+        if max_new_tokens > max(room, 0) and (eos_token_id is None or room < 1):
+            raise ValueError(f"{prompt.shape[1]} + {max_new_tokens} - 1 positions exceed the cache capacity "
+                             f"{self.capacity}")
+        max_new_tokens = min(max_new_tokens, room)
         P, K = prompt.shape[0], num_beams
         self.reset()
         seqs = torch.empty(P, K, 0, dtype=torch.long, device=self.device)
