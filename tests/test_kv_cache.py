@@ -382,3 +382,24 @@ def test_fused_step_bounded_wait_runs_out_and_recovers():
     assert (got - want).abs().max().item() <= 2e-2 * max(1.0, want.abs().max().item())
     with pytest.raises(RuntimeError):
         _lib.check(lib.tk_decode_step_withhold_arrival(scratch, -2), "tk_decode_step_withhold_arrival")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("S", [1, 100])
+def test_own_cache_objects(S):
+    """An object with ``k``, ``v`` and ``workspace`` serves the attention module as a layer of ``KVCache`` does."""
+    require_b200()
+    import tinker_b200
+
+    class Own:
+        def __init__(self, layer):
+            self.k, self.v, self.workspace = layer.k, layer.v, layer.workspace
+
+    torch.manual_seed(0)
+    attn = tinker_b200.TinKerAttention(256, 4, 2, max_seq_len=128).cuda().half()
+    x = torch.randn(2, S, 256, device="cuda").half()
+    caches = [tinker_b200.KVCache(1, 2, 4, 2, 64, 128) for _ in range(2)]
+    with torch.inference_mode():
+        a = attn(x, kv_cache=caches[0].layer(0))
+        b = attn(x, kv_cache=Own(caches[1].layer(0)))
+    assert torch.equal(a, b) and torch.equal(caches[0].k, caches[1].k) and torch.equal(caches[0].v, caches[1].v)

@@ -16,6 +16,7 @@ import torch.nn as nn
 
 from tinker_b200.kernels.fused_attention import causal_attention, fused_attention, precompute_rope_tables
 from tinker_b200.kernels.gemm import linear, linear_rope
+from tinker_b200.kernels.kv_cache import kv_append, kv_attention
 from tinker_b200 import torch_ops
 from tinker_b200.modules._roles import attention_projections
 
@@ -78,9 +79,10 @@ class TinKerAttention(nn.Module):
                 kv_cache=None, position: torch.Tensor | None = None) -> torch.Tensor:
         """forward pass; with ``residual`` the o_proj epilogue adds it to the output.
 
-        ``kv_cache`` (a ``KVCacheLayer`` or ``KVCache8Layer``): x holds the tokens at positions ``start_pos ..`` (or from
-        the device int32 ``position[0]`` on), which attend to the cached positions before them and
-        are appended to the cache."""
+        ``kv_cache`` (a ``KVCacheLayer`` or ``KVCache8Layer``, or an object with the ``k``, ``v`` and
+        ``workspace`` of the former): x holds the tokens at positions ``start_pos ..`` (or from the device
+        int32 ``position[0]`` on), which attend to the cached positions before them and are appended to the
+        cache."""
         if kv_cache is not None:
             a = self.cached_attention(x, self.q_proj.weight, self.k_proj.weight, self.v_proj.weight, kv_cache,
                                       start_pos, position)
@@ -118,11 +120,18 @@ class TinKerAttention(nn.Module):
                               l2_prefetch=l2_prefetch)
             k, v = qkv[..., hq:hq + hkv], qkv[..., hq + hkv:]
             a = causal_attention(qkv[..., :hq], k, v, self.num_heads, self.num_kv_heads, self.head_dim)
-            kv_cache.append(k, v, 0)
+            if hasattr(kv_cache, "append"):
+                kv_cache.append(k, v, 0)
+            else:
+                kv_append(k, v, kv_cache.k, kv_cache.v, 0)
             return a
         qkv = linear(x, wq, wk, wv, **norm, l2_prefetch=l2_prefetch)
-        return kv_cache.attend(qkv[..., :hq], qkv[..., hq:hq + hkv], qkv[..., hq + hkv:], self.cos_table,
-                               self.sin_table, self.num_heads, self.num_kv_heads, self.head_dim, start_pos, position)
+        q, k, v = qkv[..., :hq], qkv[..., hq:hq + hkv], qkv[..., hq + hkv:]
+        if hasattr(kv_cache, "attend"):
+            return kv_cache.attend(q, k, v, self.cos_table, self.sin_table, self.num_heads, self.num_kv_heads,
+                                   self.head_dim, start_pos, position)
+        return kv_attention(q, k, v, self.cos_table, self.sin_table, kv_cache.k, kv_cache.v, self.num_heads,
+                            self.num_kv_heads, self.head_dim, start_pos, position, kv_cache.workspace(S))
 
     @classmethod
     def from_module(cls, source: nn.Module, rope_theta: float = 10000.0, max_seq_len: int = 2048) -> "TinKerAttention":
