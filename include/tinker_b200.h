@@ -223,10 +223,13 @@ TK_API int tk_kv8_append(const void* k, int64_t k_tok_stride, const void* v, int
  * position of sequence b is start_pos_device[b * start_pos_step] (step 0 or 1), read at run time; a
  * position outside the cache or the table records device error 2, leaves that sequence's cache as it
  * is and fills its rows of out with NaN. A row that sees a token whose key or value holds a NaN or an
- * infinity is NaN throughout; other rows are what they are without it. workspace: tk_kv8_attention_workspace() bytes, zero-filled; calls of any
- * shape that follow one another on a stream can share it, calls that overlap must not. One launch for
- * S = 1, two otherwise; from 64 query rows of a kv head on, at a position known on the host, four or
- * more (the operands are laid out for the tensor cores first, in the workspace).
+ * infinity is NaN throughout; other rows are what they are without it. workspace:
+ * tk_kv8_attention_workspace() bytes, zero-filled; calls of any shape that follow one another on a
+ * stream can share it, calls that overlap must not. One launch for S = 1, two otherwise. For S > 1 with
+ * 64 query rows of a kv head or more, at a position known on the host, the operands are laid out for the
+ * tensor cores in the workspace: two or three launches for each group of sequences whose operands fit in
+ * a gigabyte, and one. There the softmax's weights are rounded once, to f16's 11 bits, and for BF16
+ * results so is the rotated q; everywhere else both have 22.
  */
 TK_API int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride, const void* v,
                             int64_t v_tok_stride, void* k_cache, void* v_cache, float* scales, void* tail,
@@ -239,6 +242,11 @@ TK_API int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void* k, 
  * comes from device memory). 0: none needed or invalid sizes, -1: no device. */
 TK_API int64_t tk_kv8_attention_workspace(int batch, int num_heads, int num_kv_heads, int head_dim, int seq,
                                           int max_kv);
+
+/* Kernels that tk_kv8_attention launches for these sizes; start_pos -1: the position comes from device memory. 0:
+ * invalid sizes, -1: no device. */
+TK_API int tk_kv8_attention_launches(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int start_pos,
+                                     int dtype);
 
 /*
  * One step of beam search. For every sequence b the best num_select of

@@ -766,3 +766,32 @@ def test_rows_of_a_position_outside_the_cache_are_nan(ragged, S, d):
     assert torch.isnan(out[bad]).all() and torch.isfinite(out[~bad]).all()
     for t, o in zip(cache, was):
         assert torch.equal(t[bad].view(torch.uint8), o[bad].view(torch.uint8))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dt, B, hq, hkv, d, n, S", [("fp16", 1, 8, 2, 64, 100, 1), ("fp16", 1, 8, 2, 64, 100, 3),
+                                                     ("bf16", 1, 32, 8, 128, 2000, 130), ("fp16", 1, 32, 8, 128, 2000, 130),
+                                                     ("bf16", 8, 32, 8, 64, 40, 256), ("bf16", 16, 32, 8, 128, 20000, 16)])
+def test_launches_are_counted(dt, B, hq, hkv, d, n, S):
+    """The counter grows by the kernels that a capture of the call holds (a memset of the workspace is none of ours)."""
+    require_b200()
+    import ctypes
+    from tinker_b200 import _lib
+    from tinker_b200.kernels import kv8_attention, kv8_attention_workspace, kv8_empty
+    dtype = DTYPES[dt]
+    cache = kv8_empty(B, hkv, d, n + S, dtype)
+    q, k, v = (torch.randn(B, S, h * d, device="cuda").to(dtype) for h in (hq, hkv, hkv))
+    ws = torch.zeros(kv8_attention_workspace(B, hq, hkv, d, S, n + S), dtype=torch.uint8, device="cuda")
+
+    def call():
+        return kv8_attention(q, k, v, None, None, *cache, hq, hkv, d, start_pos=n, workspace=ws)
+    call()
+    graph = torch.cuda.CUDAGraph(keep_graph=True)
+    n0 = _lib.launch_counter[0]
+    with torch.cuda.graph(graph):
+        out = call()
+    counted = _lib.launch_counter[0] - n0
+    nodes = ctypes.c_size_t()
+    cudart = ctypes.CDLL("libcudart.so.12")
+    assert cudart.cudaGraphGetNodes(ctypes.c_void_p(graph.raw_cuda_graph()), None, ctypes.byref(nodes)) == 0
+    assert counted == nodes.value and out.shape == q.shape

@@ -77,6 +77,7 @@ SIGNATURES = {
     "tk_kv8_attention": [_P, _I64, _P, _I64, _P, _I64, _P, _P, _P, _P, _I, _I, _P, _P, _I64, _P, _I64, _I, _I, _I, _I,
                          _I, _I, _P, _I, _P, _I64, _I, _P],
     "tk_kv8_attention_workspace": [_I, _I, _I, _I, _I, _I],
+    "tk_kv8_attention_launches": [_I, _I, _I, _I, _I, _I, _I],
     "tk_beam_select": [_P, _I64, _P, _P, _I64, _P, _P, _P, _I, _I, _I, _I, _P, _I64, _I, _P],
     "tk_beam_select_workspace": [_I, _I, _I, _I, _I],
     "tk_kv_reorder": [_P, _P, _P, _I, _I, _I, _I, _I, _I, _I, _P, _I, _P],

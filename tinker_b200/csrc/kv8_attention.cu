@@ -972,6 +972,18 @@ extern "C" int64_t tk_kv8_attention_workspace(int batch, int num_heads, int num_
   return need;
 }
 
+extern "C" int tk_kv8_attention_launches(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int start_pos,
+                                         int dtype) {
+  using namespace tk;
+  if (batch <= 0 || seq <= 0 || num_heads <= 0 || num_kv_heads <= 0 || num_heads % num_kv_heads) return 0;
+  if (seq == 1) return 1;
+  const int64_t len = int64_t(start_pos) + seq;
+  if (start_pos < 0 || !kv8::chunk_fits(batch, num_heads, num_kv_heads, seq, len)) return 2;
+  DeviceInfo di;
+  if (current_device_info(&di)) return -1;
+  return kv8::chunk_launches(batch, num_heads, num_kv_heads, head_dim, seq, len, dtype, di.sm_count) + 1;
+}
+
 extern "C" int tk_kv8_attention(const void* q, int64_t q_tok_stride, const void* k, int64_t k_tok_stride,
                                 const void* v, int64_t v_tok_stride, void* k_cache, void* v_cache, float* scales,
                                 void* tail, int num_blocks, int format, const float* cos_table,

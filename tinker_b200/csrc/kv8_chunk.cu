@@ -757,6 +757,18 @@ int64_t chunk_workspace(int batch, int num_heads, int num_kv_heads, int head_dim
   return n < batch ? std::max(here, int64_t(1) << 30) : here;
 }
 
+int chunk_launches(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int64_t len, int dtype,
+                   int sm_count) {
+  const int64_t rows = int64_t(num_heads / num_kv_heads) * seq;
+  const int at_once = sequences_at_once(batch, num_kv_heads, rows, len, head_dim, sm_count);
+  int n = 0;
+  for (int b = 0; b < batch; b += at_once) {
+    const int m = std::min(at_once, batch - b);
+    n += chunk::make_plan(m, num_kv_heads, rows, len, head_dim, dtype == TK_F16, sm_count).splits > 1 ? 3 : 2;
+  }
+  return n;
+}
+
 int chunk_attention(const Cache& c, const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs,
                     const float* cos_t, const float* sin_t, void* out, int64_t os, int batch, int seq, int num_heads,
                     int num_kv_heads, int head_dim, int start_pos, void* workspace, int dtype, int sm_count,

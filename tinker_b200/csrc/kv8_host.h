@@ -30,6 +30,8 @@ int append(const Cache& c, const void* k, int64_t ks, const void* v, int64_t vs,
 constexpr int CHUNK_MIN_ROWS = 64;  // query rows of a kv head, of two new tokens or more
 bool chunk_fits(int batch, int num_heads, int num_kv_heads, int seq, int64_t len);
 int64_t chunk_workspace(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int64_t len, int sm_count);
+int chunk_launches(int batch, int num_heads, int num_kv_heads, int head_dim, int seq, int64_t len, int dtype,
+                   int sm_count);
 int chunk_attention(const Cache& c, const void* q, int64_t qs, const void* k, int64_t ks, const void* v, int64_t vs,
                     const float* cos_t, const float* sin_t, void* out, int64_t os, int batch, int seq, int num_heads,
                     int num_kv_heads, int head_dim, int start_pos, void* workspace, int dtype, int sm_count,

@@ -70,6 +70,13 @@ def _workspace_bytes(idx: int, *sizes) -> int:
         return kv8_attention_workspace(*sizes)
 
 
+@functools.lru_cache(maxsize=256)
+def _launches(idx: int, *sizes) -> int:
+    """Kernels that a call on device ``idx`` launches."""
+    with torch.cuda.device(idx):
+        return _lib.lib().tk_kv8_attention_launches(*sizes)
+
+
 def _rows(t: torch.Tensor, B: int, S: int, width: int) -> tuple[torch.Tensor, int]:
     """(tensor, token stride) of [B, S, width] rows that start on 16 bytes and follow one another at one
     stride; anything else is copied."""
@@ -116,7 +123,9 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
     kernel runs (one CUDA graph serves every step); a position outside the cache or the tables then
     records device error 2, leaves that sequence's cache untouched and gives rows of NaN for it. Keys of complete blocks
     are read as ``code * scale``, those of the open block and of this call in 16 bits. A row that sees a
-    token whose key or value holds a NaN or an infinity is NaN throughout. ``workspace``:
+    token whose key or value holds a NaN or an infinity is NaN throughout. q and the softmax's weights are
+    products in two parts of 11 bits; from 64 query rows of a kv head on (S > 1, position on the host) on
+    tensor-core tiles, where the weights are rounded to 11 bits, and q too for bfloat16. ``workspace``:
     zero-filled uint8 CUDA tensor of at least ``kv8_attention_workspace(...)`` bytes, left so that
     later calls of any shape can use it, but not calls that overlap in time (allocated per call when
     omitted). Returns [B, S, num_heads * head_dim] in q's dtype.
@@ -166,7 +175,10 @@ def kv8_attention(q, k, v, cos_table, sin_table, k_cache, v_cache, scales, tail,
         workspace = (torch.empty if need > base else torch.zeros)(need, dtype=torch.uint8, device=out.device)
     elif workspace.nbytes < need or workspace.get_device() != idx or not workspace.is_contiguous():
         raise ValueError(f"kv8_attention: workspace smaller than the {need} bytes needed, or not contiguous")
-    launch(idx, "tk_kv8_attention", 1 if S == 1 else 2, _lib.lib().tk_kv8_attention, q.data_ptr(), qs, k.data_ptr(), ks,
+    kernels = 1 if S == 1 else 2
+    if need > base:
+        kernels = _launches(idx, B, num_heads, num_kv_heads, head_dim, S, start_pos, _lib.dtype_code(dtype))
+    launch(idx, "tk_kv8_attention", kernels, _lib.lib().tk_kv8_attention, q.data_ptr(), qs, k.data_ptr(), ks,
            v.data_ptr(), vs, k_cache.data_ptr(), v_cache.data_ptr(), scales.data_ptr(), tail.data_ptr(), nb, code,
            cos_ptr, sin_ptr, rows, out.data_ptr(), width, B, S, num_heads, num_kv_heads, head_dim, start_pos, pos_ptr,
            step, workspace.data_ptr(), need, _lib.dtype_code(dtype))
