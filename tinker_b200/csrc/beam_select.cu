@@ -17,14 +17,21 @@
 //      the value of the n-th best so far; vectors that hold a larger one are put aside and, every STRIDE vectors,
 //      ranked with the best n, which raises the threshold. Equal elements that come later lose in any case.
 //      An exponential is 2^(x L - b) with L = log2 e and b = m L rounded; the sum is corrected by 2^(b - m L), the
-//      rounding that all its terms share. Where the reference proves too far off (a masked beginning) or is above 2^20 (the
-//      rounding grows with it), the sum is taken again. A segment with a NaN or +inf, or with more candidates than the lists hold, is done again in the
-//      plain way: cleaned, its maximum, the sum of e^(x - m), n rounds of a maximum over (value, index).
+//      rounding that all its terms share. Where the reference proves too far off (a masked beginning) or is above 2^20
+//      (the rounding grows with it), the sum is taken again. A segment with a NaN or +inf, or with more candidates than
+//      the lists hold, is done again in the plain way: cleaned, its maximum, the sum of e^(x - m), n rounds of a maximum
+//      over (value, index).
 //   2. a CTA for each sequence joins the segments' sums to a logsumexp for each beam, takes a threshold from the heads of
 //      the segments' lists in the same way, walks each list down to it and ranks what it finds, with c in fp64.
 // Sums are taken in an order that depends on element numbers alone, so equal rows give equal sums wherever they lie.
-// Bound by the instructions of the first launch for many rows (256 rows of 151936, a quarter finished: 28.4 us; the
-// logits alone 8.9 us, the exponentials 7 us), by the latency of the two launches for few (4 rows of 32000: 9.7 us).
+// For many rows bound by the first launch's order: its CTAs all fit at once and go through the same prologue (load,
+// threshold, collect, rank) together, so that 57 % of the issue slots are filled and the logits come at 2.7 TB/s (256
+// rows of 151936, a quarter finished: 28.5 us; the logits alone 8.9 us, the exponentials 7 us, all instructions 11 us;
+// all live 38.4 us, fp32 53.7 us). For few by the latency of the two launches (4 rows of 32000: 9.4 us).
+// Slow, not wrong: rows that do not begin on 16 bytes (an odd vocabulary, for 7 of 8 rows of 16-bit logits) are read
+// element by element (256 rows of 50257: 33.4 us, of 50264: 25.7 us); a round of STRIDE steps with more than HITS vectors
+// above the threshold (a masked beginning of 8192 16-bit logits before unmasked ones, steadily rising logits) sends the
+// segment to the plain way (256 rows of 151936: 900 us).
 #include <math.h>
 
 #include <algorithm>
@@ -147,7 +154,7 @@ struct ChunkSmem {
 // A segment in the plain way, element tid, tid + THREADS, ... for a thread.
 template <int DT>
 __device__ __forceinline__ void plain_segment(const Params& p, const typename Logit<DT>::T* src, int lo, int hi,
-                                           int64_t part, ChunkSmem& sm) {
+                                              int64_t part, ChunkSmem& sm) {
   constexpr float TOP = DT == TK_F16 ? 65504.f : DT == TK_BF16 ? 3.3895313892515355e38f : 3.4028234663852886e38f;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   auto get = [&](int at) { return fminf(fmaxf(Logit<DT>::to_f(src[at]), -INFINITY), TOP); };  // fmaxf turns NaN into -inf
@@ -174,8 +181,8 @@ __device__ __forceinline__ void plain_segment(const Params& p, const typename Lo
 #pragma unroll 1
   for (int i = 0; i < p.n; ++i) {
     ulonglong2 v = make_ulonglong2(0, 0);
-  #pragma unroll 1
-  for (int at = lo + tid; at < hi; at += THREADS) {
+#pragma unroll 1
+    for (int at = lo + tid; at < hi; at += THREADS) {
       const uint64_t k = key_of(get(at)), t = static_cast<uint32_t>(~at);
       if ((k < last.x || (k == last.x && t < last.y)) && (k > v.x || (k == v.x && t > v.y))) v = make_ulonglong2(k, t);
     }
@@ -232,7 +239,8 @@ __global__ void __launch_bounds__(THREADS, 4) beam_chunk_kernel(const Params p) 
   pdl_launch_dependents();
   if (is_still(p, row)) return;
   const T* src = static_cast<const T*>(p.logits) + static_cast<int64_t>(row) * p.row_stride;
-  const int lo = split * p.segment, hi = static_cast<int>(min(static_cast<int64_t>(p.vocab), static_cast<int64_t>(lo) + p.segment));
+  const int lo = split * p.segment;
+  const int hi = static_cast<int>(min(static_cast<int64_t>(p.vocab), static_cast<int64_t>(lo) + p.segment));
   const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0;
   const int64_t part = static_cast<int64_t>(row) * p.splits + split;
 
@@ -578,8 +586,8 @@ __global__ void __launch_bounds__(THREADS) beam_merge_kernel(const Params p) {
       c = done && j == 0 ? static_cast<double>(f.z) : -INFINITY;
     } else {
       const float x = __int_as_float(t.x);
-      c = x == -INFINITY ? -INFINITY
-                         : static_cast<double>(f.z) + ((static_cast<double>(x) - static_cast<double>(f.x)) - static_cast<double>(f.y));
+      const double below = static_cast<double>(x) - static_cast<double>(f.x) - static_cast<double>(f.y);
+      c = x == -INFINITY ? -INFINITY : static_cast<double>(f.z) + below;
     }
     at = static_cast<uint64_t>(k) << 32 | static_cast<uint32_t>(token);
     return token >= 0;

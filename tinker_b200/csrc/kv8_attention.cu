@@ -25,9 +25,11 @@
 // for a tile of 64 columns and four rows, twice the accumulators, and 20.5 us instead of 18.7 us for 64 sequences of 4
 // kv heads at 2047.)
 //
-// Bound by HBM at D = 128 (16 x 16001 positions of 8 kv heads: 87 us, 6.0 TB/s), at D = 64 by the instructions of a tile
-// as much (48 ragged sequences of 8 kv heads: 45.6 us, 4.5 TB/s; int8 costs 97 instructions more than e4m3), for
-// little work by the chain position - copies - products - merge (7 us for one sequence of 4 kv heads at 127).
+// Bound by HBM at D = 128 (16 x 16001 positions of 8 kv heads: 87 us, 6.0 TB/s). At D = 64 by latency and balance: a warp
+// goes copies - products - maximum - products tile by tile, and the instructions fill a third to a half of the issue slots
+// (64 x 2047 of 4 kv heads, one CTA a unit: 18.6 us, 31 %; 48 ragged sequences of 8 kv heads, int8: 45.6 us, 4.5 TB/s, 45 %;
+// 2 x 100003 with 7 heads a kv head, int8: 26.6 us, 28 %). For little work by the chain position - copies - products - merge
+// (7 us for one sequence of 4 kv heads at 127). int8 costs some 97 instructions a tile more than e4m3.
 //
 // Division of the work: all units' tiles in one line (beginning a unit counts UNIT_WEIGHT, a 16-bit tile TAIL_WEIGHT),
 // cut into equal pieces, one for each warp that fits on the GPU at once. So long and short sequences, few units and

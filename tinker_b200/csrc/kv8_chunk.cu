@@ -11,18 +11,20 @@
 //    Codes and scaled rows are exact in f16; q is rounded to 11 bits, 2^-12 of each of a score's terms. Under a bf16
 //    result (2^-9) that does not show; for an fp16 result it would double the error (4.3e-4 instead of 2.1e-4 relative
 //    on 8-bit keys with strong channels), so there the remainder q - f16(q) is laid out too and has a product of its
-//    own. The weights are rounded to f16 once, 2^-12 of a weight, in both. They go up to 2^15, so one is
-//    lost to f16's smallest number, 2^-24, only 2^36 below the largest.
-// 2. kv8_chunk_kernel: a CTA takes two 128-row query tiles (fp16: one and its remainder) of one (sequence, kv head) - rows of all the heads that
-//    share it, so a key tile is loaded once for them - and a range of the 128-key tiles. One thread feeds a ring of K
-//    and V tiles by TMA, one issues S = Q K^T and O += P V as tcgen05.mma with S and O in tensor memory, two
-//    warpgroups (thread = query row) turn S into weights: x = s * (factor * scale_k) + log2 scale_v for each 32 keys, w =
-//    2^(x - m + HEADROOM), l += sum w / scale_v, P = f16(w) to shared memory. m moves only when a tile raises it by more than
-//    2^4. The scales cost nothing per score: the FMA of the softmax takes them as its factor and addend.
+//    own. The weights are rounded to f16 once, 2^-12 of a weight, in both. They go up to 2^15, so one is lost to f16's
+//    smallest number, 2^-24, only 2^36 below the largest.
+// 2. kv8_chunk_kernel: a CTA takes two 128-row query tiles (fp16: one and its remainder) of one (sequence, kv head) -
+//    rows of all the heads that share it, so a key tile is loaded once for them - and a range of the 128-key tiles. One
+//    thread feeds a ring of K and V tiles by TMA, one issues S = Q K^T and O += P V as tcgen05.mma with S and O in
+//    tensor memory, two warpgroups (thread = query row) turn S into weights: x = s * (factor * scale_k) + log2 scale_v
+//    for each 32 keys, w = 2^(x - m + HEADROOM), l += sum w / scale_v, P = f16(w) to shared memory. m moves only when a
+//    tile raises it by more than 2^4. The scales cost nothing per score: the FMA of the softmax takes them as its factor
+//    and addend.
 // 3. With the key axis split (few query tiles), kv8_join_kernel merges the parts in their order.
 // Bound by the softmax's latency: products and exponentials take some 2000 cycles each for a pair of tiles at D = 128, a
-// step some 6000 (8 softmax warps on 4 schedulers). 512 tokens of 32 heads of 128 at 7001: 129 us in all, 100 of them
-// here (128 CTAs), the rest the expansion, the join and the append; 160 us for fp16. kv8_attention.cu took 641 us.
+// step some 6000 (8 softmax warps on 4 schedulers, 29 % of the issue slots filled). 512 tokens of 32 heads of 128 at
+// 7001: 124 us in all, 100 of them here (128 CTAs), the rest the expansion, the join and the append; 154 us for fp16,
+// whose second warpgroup has no tile. kv8_attention.cu takes 739 us.
 #include <algorithm>
 #include <cmath>
 #include <string>
@@ -247,11 +249,12 @@ __global__ void __launch_bounds__(EXPAND_WARPS * 32, 2) kv8_expand_kernel(const 
   uint32_t amax = amax2_warp(m), bad = 0;
   __syncwarp();
   if (amax >= not_finite_bits<DT>()) {
-    // A token that is not finite makes the rows that see it NaN, by its scores, and must not reach the others, neither as 0 *
-    // NaN nor by the range of its 32 tokens: a key becomes NaN throughout, values become 0 and their bit does the same.
+    // A token that is not finite makes the rows that see it NaN, by its scores, and must not reach the others, neither as
+    // 0 * NaN nor by the range of its 32 tokens: a key becomes NaN throughout, values become 0 and their bit does the same.
 #pragma unroll 1
     for (int idx = lane; idx < BLOCK * C16; idx += 32)
-      if (not_finite<DT>(*reinterpret_cast<const uint4*>(tile + tile_off<D>(idx / C16, idx % C16)))) bad |= 1u << (idx / C16);
+      if (not_finite<DT>(*reinterpret_cast<const uint4*>(tile + tile_off<D>(idx / C16, idx % C16))))
+        bad |= 1u << (idx / C16);
     bad = __reduce_or_sync(0xffffffffu, bad);
     const uint32_t w = values ? 0u : 0x7fff7fffu;
     m = 0;
@@ -691,7 +694,8 @@ template <int DT, int FMT, int D>
 int launch(Params& p, const Plan& pl, cudaStream_t st) {
   const uint64_t bh = uint64_t(p.batch) * p.num_kv_heads;
   CUtensorMap tq, tk_, tv;
-  if (int rc = tensor_map_3d(&tq, p.qx, TK_F16, D, p.rows, REMAINDER<DT> ? 2 * bh : bh, D, uint64_t(p.rows) * D, 64, BQ, 1)) return rc;
+  const uint64_t q_parts = REMAINDER<DT> ? 2 * bh : bh;
+  if (int rc = tensor_map_3d(&tq, p.qx, TK_F16, D, p.rows, q_parts, D, uint64_t(p.rows) * D, 64, BQ, 1)) return rc;
   if (int rc = tensor_map_3d(&tk_, p.kx, TK_F16, D, p.keys, bh, D, uint64_t(p.keys) * D, 64, BKV, 1)) return rc;
   if (int rc = tensor_map_3d(&tv, p.vx, TK_F16, p.keys, D, bh, p.keys, uint64_t(p.keys) * D, 64, D, 1)) return rc;
   auto kern = kv8_chunk_kernel<DT, D>;
@@ -715,8 +719,9 @@ int launch(Params& p, const Plan& pl, cudaStream_t st) {
   if (int rc = launch_kernel(expand, dim3(p.q_ctas + k_ctas, p.num_kv_heads, p.batch), dim3(EXPAND_WARPS * 32),
                              EXPAND_SMEM, st, 1, "kv8_expand", p))
     return rc;
-  if (int rc = launch_kernel(kern, dim3(p.num_kv_heads, p.batch, (REMAINDER<DT> ? p.n_qtiles : (p.n_qtiles + 1) / 2) * p.splits), dim3(THREADS),
-                             Smem<D>::TOTAL, st, 1, "kv8_chunk", tq, tk_, tv, p))
+  const int query_ctas = REMAINDER<DT> ? p.n_qtiles : (p.n_qtiles + 1) / 2;
+  if (int rc = launch_kernel(kern, dim3(p.num_kv_heads, p.batch, query_ctas * p.splits), dim3(THREADS), Smem<D>::TOTAL, st, 1,
+                             "kv8_chunk", tq, tk_, tv, p))
     return rc;
   if (p.splits == 1) return TK_OK;
   return launch_kernel(kv8_join_kernel<DT, D>, dim3((p.rows + 7) / 8, p.num_kv_heads, p.batch), dim3(256), 0, st, 1,
